@@ -667,6 +667,58 @@ int ctr_covis_row_features(const int64_t* rows, long nq, const int64_t* row_ptr,
                            const uint64_t* keys, const double* ctr, const int32_t* impr, const int64_t* n_pairs,
                            int topn, double* out, void* stream);
 
+/* ---- layer norm of fp32 / bf16 / fp16 rows, forward and backward                                   (ln.hip)
+ * Types: 0 fp32, 1 bf16, 2 fp16.  xt: x, y, dy, dx; wt: w, b, dw, db -- fp32 or the rows' type.  Statistics and sums are
+ * fp32.  b, db nullable.  mean / rstd (M) are written by the forward and read by the backward.  Row strides in
+ * elements; rows of any width start at any element.  dw / db are the whole sums over the rows, in the weight's type
+ * (zeros for M = 0), the same bits every time.                                                           */
+int ctr_ln_fwd(const void* x, long ldx, long M, int N, const void* w, const void* b, float eps, void* y, long ldy,
+               float* mean, float* rstd, int xt, int wt, void* stream);
+size_t ctr_ln_bwd_ws_size(long M, int N);
+int ctr_ln_bwd(const void* dy, long lddy, const void* x, long ldx, const float* mean, const float* rstd, const void* w,
+               long M, int N, void* dx, long lddx, void* dw, void* db, void* ws, size_t ws_bytes, int xt, int wt,
+               void* stream);
+
+/* ---- differential attention: O = (softmax(Q1 K1^T scale) - lam softmax(Q2 K2^T scale)) V        (diffattn.hip)
+ * q (B, T, H, 2, D), k (B, S, Hkv, 2, D), v (B, S, Hkv, 2 D) of type 1 bf16 / 2 fp16, D in {32, 64, 128}, element strides
+ * as given (multiples of 8, 16-byte aligned rows, the last axis contiguous); lam (H) fp32; H a multiple of Hkv (a key
+ * head serves H / Hkv consecutive query heads).  o (B, T, H, 2 D) contiguous.  q_lens / kv_lens (B) nullable: valid
+ * positions and keys of each sequence, held to [0, T] / [0, S]; what stands behind
+ * kv_lens does not count.  causal: position t sees the keys up to t + kv_len - q_len.  A row that sees no key, and a position behind q_len, gives zeros (and zero
+ * gradients).  For the backward pass o2 (the shape of o: the second map's part) and stat (4 * B * H * T floats: the
+ * rows' log-sums, and space for the backward's row sums) are written by the forward; both null: inference.
+ * ctr_diffattn_bwd: dout (B, T, H, 2 D) with strides; dq, dk, dv contiguous in the shapes of q, k, v; dlam (H) fp32.  */
+typedef struct {
+  const void *q, *k, *v;
+  const float* lam;
+  void *o, *o2;
+  float* stat;
+  const int32_t *q_lens, *kv_lens;
+  long q_sb, q_st, q_sh, q_sc, k_sb, k_ss, k_sh, k_sc, v_sb, v_ss, v_sh;
+  float scale;
+  int B, T, S, H, Hkv, D, causal, type;
+} ctr_diffattn_t;
+size_t ctr_diffattn_fwd_ws_size(const ctr_diffattn_t* p);
+int ctr_diffattn_fwd(const ctr_diffattn_t* p, void* ws, size_t ws_bytes, void* stream);
+size_t ctr_diffattn_bwd_ws_size(const ctr_diffattn_t* p);
+int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long g_sb, long g_st, long g_sh, void* dq, void* dk, void* dv,
+                     float* dlam, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- Newton-Schulz orthogonalisation of a list of matrices                                    (newton_schulz.hip)
+ * X_0 = G / (||G||_F + eps); `steps` times X <- (a I + b A + c A^2) X, A = X X^T (of the transpose when there are more rows
+ * than columns).  src / dst of type 0 fp32, 1 bf16, 2 fp16, row strides in elements; computed to fp32's accuracy.
+ * The list is host memory and is read during the call only.  Coefficients under which a singular value could leave
+ * [0, 7.5] are refused.                                                                                  */
+typedef struct {
+  const void* src;
+  void* dst;
+  long ld_src, ld_dst;
+  int rows, cols;
+} ctr_ns_mat_t;
+size_t ctr_newton_schulz_ws_size(const ctr_ns_mat_t* mats, int count);
+int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps, float a, float b, float c, float eps, int type,
+                      void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,673 @@
+// Newton-Schulz orthogonalisation of matrices (the direction of a Muon update) and the update around it.
+//   X_0 = G / (||G||_F + eps)  (transposed when it has more rows than columns: m <= n below)
+//   A = X X^T,   W = a I + b A + c A^2,   X <- W X        (`steps` times)
+//
+// Arithmetic.  X, A and W are kept as two fp16 planes, hi = fp16(s v) and lo = fp16(s v - hi) with s a power of two that
+// keeps lo out of fp16's subnormals (X: 2^12, A and W: 2^10; the host refuses coefficients under which a singular value
+// of X could pass 8 or one of W 32, the planes' range): 22 mantissa bits and a sign of lo, which is fp32's step to within
+// a factor of two.  A product of two such values is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 with fp32
+// accumulation; the lo lo term is 2^-24 of it.  Three fp16 products cost 3/16 of one fp32 matrix instruction's time, so
+// this is fp32's accuracy at up to five times its rate.  16-bit accuracy would not do: the polynomial multiplies the error
+// of a small singular value by a (3.44) a step, 485 times in five.  The squares of the norm are summed in fp64, where no
+// fp32 input overflows or vanishes.
+#include <algorithm>
+#include <atomic>
+
+#include "ctr_hip.h"
+#include "vec16.h"
+
+namespace ctr {
+namespace {
+
+constexpr float SX = 4096.f, SA = 1024.f;      // the planes' scales of X and of A, W
+constexpr int NS_MAXMAT = 20;                  // matrices of one launch (their table rides in the kernel arguments)
+constexpr int NS_TILE = 128, NS_BK = 32;
+constexpr int LDK = NS_BK + 8, LDN = NS_TILE + 32;   // LDS row strides (elements): k-contiguous tiles, n-contiguous tiles
+constexpr int PLANE_K = NS_TILE * LDK, PLANE_N = NS_BK * LDN;
+static_assert(PLANE_K == PLANE_N, "one LDS plane size");
+constexpr int NS_SUMSQ_BLOCKS = 64;
+constexpr int NS_SMALL_LDS = 160 * 1024 - 256;   // of a workgroup, next to its few static bytes
+
+struct NsMat {
+  const void* src;
+  void* dst;
+  long ld_src, ld_dst;
+  int rows, cols;          // as given
+  int m, n, mp, np;        // m <= n, and both rounded up to the tile
+  long off_x, off_a, off_p, off_s;     // bytes into the workspace: X planes (two buffers), A / W planes, Gram partials, sums
+  int splits, type;
+};
+struct NsArgs {
+  int count;
+  int pre[NS_MAXMAT + 1];  // first block of each matrix
+  char* ws;
+  float a, b, c, eps;
+  NsMat mat[NS_MAXMAT];
+};
+
+__device__ __forceinline__ int ns_find(const NsArgs& p, int blk) {
+  int i = 0;
+  while (i + 1 < p.count && blk >= p.pre[i + 1]) ++i;
+  return i;
+}
+
+__device__ __forceinline__ float ns_load(const NsMat& q, int r, int c) {
+  const long o = (long)r * q.ld_src + c;
+  return q.type == TY_F32 ? ((const float*)q.src)[o] : q.type == TY_BF16 ? (float)((const __bf16*)q.src)[o]
+                                                                         : (float)((const _Float16*)q.src)[o];
+}
+__device__ __forceinline__ void ns_store(const NsMat& q, int r, int c, float v) {
+  const long o = (long)r * q.ld_dst + c;
+  if (q.type == TY_F32) ((float*)q.dst)[o] = v;
+  else if (q.type == TY_BF16) ((__bf16*)q.dst)[o] = (__bf16)v;
+  else ((_Float16*)q.dst)[o] = (_Float16)v;
+}
+
+__device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  lo = (_Float16)(v - (float)hi);
+}
+
+__device__ __forceinline__ double block_sum64(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[i];
+  return s;
+}
+
+// C layout of a 32x32 tile: register r of lane l holds row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32
+__device__ __forceinline__ int c_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+#define MFMA16(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_f16(A, B, C, 0, 0, 0)
+
+typedef __attribute__((address_space(3))) f16x4 lds_f16x4;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Fragment of 32 rows x 16 k from rows with contiguous k: lane l has row l % 32, k = 8 (l / 32) + 0..7
+__device__ __forceinline__ f16x8 frag_k(const _Float16* p, int ld, int row, int k, int lane) {
+  return *(const f16x8*)(p + (row + (lane & 31)) * ld + k + 8 * (lane >> 5));
+}
+// The same rows with the k order that frag_t gives: 4 (l / 32) + 0..3, then 8 + 4 (l / 32) + 0..3
+__device__ __forceinline__ f16x8 frag_kp(const _Float16* p, int ld, int row, int k, int lane) {
+  const _Float16* q = p + (row + (lane & 31)) * ld + k + 4 * (lane >> 5);
+  const f16x4 u = *(const f16x4*)q, v = *(const f16x4*)(q + 8);
+  return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Fragment of 16 k x 32 columns from rows of contiguous columns, by the LDS transpose read: a group of 16 lanes takes
+// 4 k rows of 16 columns, lane i of it the address of row i / 4, columns 4 (i % 4), and gets column i's four k
+__device__ __forceinline__ f16x8 frag_t(const _Float16* p, int ld, int k, int col, int lane) {
+  const int row = k + 4 * (lane >> 5) + ((lane & 15) >> 2), c = col + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  auto q = (__attribute__((address_space(3))) s16x4*)(p + row * ld + c);
+  auto q8 = (__attribute__((address_space(3))) s16x4*)(p + (row + 8) * ld + c);
+  const f16x4 u = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q));
+  const f16x4 v = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q8));
+  return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// ------------------------------------------------------------------------------------------------ large matrices
+__global__ __launch_bounds__(256) void ns_sumsq(const NsArgs p) {
+  const NsMat& q = p.mat[blockIdx.y];
+  __shared__ double red[4];
+  double s = 0.;
+  const long total = (long)q.rows * q.cols;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const int r = (int)(i / q.cols), c = (int)(i - (long)r * q.cols);
+    const double v = ns_load(q, r, c);
+    s = fma(v, v, s);
+  }
+  s = block_sum64(s, red);
+  if (threadIdx.x == 0) ((double*)(p.ws + q.off_s))[blockIdx.x] = s;
+}
+
+// X_0's planes, 64 x 64 elements a block, through LDS when transposed
+__global__ __launch_bounds__(256) void ns_init(const NsArgs p) {
+  const int i = ns_find(p, blockIdx.x);
+  const NsMat& q = p.mat[i];
+  __shared__ double red[4];
+  __shared__ float tile[64][65];
+  const double part = threadIdx.x < NS_SUMSQ_BLOCKS ? ((const double*)(p.ws + q.off_s))[threadIdx.x] : 0.;
+  const float scale = (float)(SX / (sqrt(block_sum64(part, red)) + (double)p.eps));
+  const int id = blockIdx.x - p.pre[i], tc = q.np / 64, m0 = id / tc * 64, n0 = id % tc * 64;
+  const bool tall = q.rows > q.cols;
+  const int lx = threadIdx.x & 63, ly = threadIdx.x >> 6;
+  for (int j = ly; j < 64; j += 4) {
+    const int r = tall ? n0 + j : m0 + j, c = tall ? m0 + lx : n0 + lx;
+    tile[j][lx] = r < q.rows && c < q.cols ? ns_load(q, r, c) : 0.f;
+  }
+  __syncthreads();
+  _Float16* x = (_Float16*)(p.ws + q.off_x);
+  const long plane = (long)q.mp * q.np;
+  for (int j = ly; j < 64; j += 4) {
+    const float v = tall ? tile[lx][j] : tile[j][lx];
+    const long o = (long)(m0 + j) * q.np + n0 + lx;
+    split16(v * scale, x[o], x[plane + o]);
+  }
+}
+
+// One 128 x 128 tile of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.
+// Four waves of 64 x 64; the next step's tiles are loaded to registers under this step's products.
+template <bool NN>
+__device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda, const _Float16* B, long planeB, int ldb,
+                                        int r0, int c0, int k0, int k1, _Float16* lds, f32x16 acc[2][2]) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+  f16x8 ra[4], rb[4];
+  const auto fetch = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int id = t + (j & 1) * 256;
+      ra[j] = *(const f16x8*)(A + (j >> 1) * planeA + (long)(r0 + id / 4) * lda + k + id % 4 * 8);
+      rb[j] = NN ? *(const f16x8*)(B + (j >> 1) * planeB + (long)(k + id / 16) * ldb + c0 + id % 16 * 8)
+                 : *(const f16x8*)(B + (j >> 1) * planeB + (long)(c0 + id / 4) * ldb + k + id % 4 * 8);
+    }
+  };
+  const auto put = [&](_Float16* s) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int id = t + (j & 1) * 256;
+      *(f16x8*)(s + (j >> 1) * PLANE_K + id / 4 * LDK + id % 4 * 8) = ra[j];
+      if (NN) *(f16x8*)(s + (2 + (j >> 1)) * PLANE_K + id / 16 * LDN + id % 16 * 8) = rb[j];
+      else *(f16x8*)(s + (2 + (j >> 1)) * PLANE_K + id / 4 * LDK + id % 4 * 8) = rb[j];
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = 0.f;
+  if (k0 >= k1) return;
+  fetch(k0);
+  put(lds);
+  __syncthreads();
+  int cur = 0;
+  for (int k = k0; k < k1; k += NS_BK) {
+    const bool more = k + NS_BK < k1;
+    if (more) fetch(k + NS_BK);
+    const _Float16* s = lds + cur * 4 * PLANE_K;
+#pragma unroll
+    for (int kk = 0; kk < NS_BK; kk += 16) {
+      f16x8 a[2][2], b[2][2];      // [plane][tile]
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          a[pl][i] = NN ? frag_kp(s + pl * PLANE_K, LDK, wr + 32 * i, kk, lane)
+                        : frag_k(s + pl * PLANE_K, LDK, wr + 32 * i, kk, lane);
+          b[pl][i] = NN ? frag_t(s + (2 + pl) * PLANE_K, LDN, kk, wc + 32 * i, lane)
+                        : frag_k(s + (2 + pl) * PLANE_K, LDK, wc + 32 * i, kk, lane);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          acc[i][j] = MFMA16(a[1][i], b[0][j], acc[i][j]);
+          acc[i][j] = MFMA16(a[0][i], b[1][j], acc[i][j]);
+          acc[i][j] = MFMA16(a[0][i], b[0][j], acc[i][j]);
+        }
+    }
+    if (more) put(lds + (cur ^ 1) * 4 * PLANE_K);
+    __syncthreads();
+    cur ^= 1;
+  }
+}
+
+// tile of the lower triangle, row by row
+__device__ __forceinline__ void tri(int id, int& ti, int& tj) {
+  ti = (int)((sqrtf(8.f * id + 1.f) - 1.f) * 0.5f);
+  while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+  while (ti * (ti + 1) / 2 > id) --ti;
+  tj = id - ti * (ti + 1) / 2;
+}
+
+// Gram partials: A = X X^T over a share of the columns, lower tiles
+__global__ __launch_bounds__(256, 2) void ns_gram(const NsArgs p, int buf) {
+  extern __shared__ __align__(16) _Float16 lds[];
+  const int i = ns_find(p, blockIdx.x);
+  const NsMat& q = p.mat[i];
+  const int id = blockIdx.x - p.pre[i], nt = q.mp / NS_TILE, tiles = nt * (nt + 1) / 2, sp = id / tiles;
+  int ti, tj;
+  tri(id % tiles, ti, tj);
+  const int steps = q.np / NS_BK, per = (steps + q.splits - 1) / q.splits;
+  const long plane = (long)q.mp * q.np;
+  const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
+  f32x16 acc[2][2];
+  ns_tile<false>(x, plane, q.np, x, plane, q.np, ti * NS_TILE, tj * NS_TILE, min(steps, sp * per) * NS_BK,
+                 min(steps, (sp + 1) * per) * NS_BK, lds, acc);
+  float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        out[(long)(ti * NS_TILE + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * NS_TILE + (wave & 1) * 64 +
+            b * 32 + (lane & 31)] = acc[a][b][r];
+}
+
+// the partials of a 32 x 32 block of the lower tiles summed in order, both triangles' planes written
+__global__ __launch_bounds__(256) void ns_gram_join(const NsArgs p) {
+  const int i = ns_find(p, blockIdx.x);
+  const NsMat& q = p.mat[i];
+  __shared__ float tile[32][33];
+  int ti, tj;
+  tri(blockIdx.x - p.pre[i], ti, tj);
+  const float* in = (const float*)(p.ws + q.off_p);
+  _Float16* A = (_Float16*)(p.ws + q.off_a);
+  const long plane = (long)q.mp * q.mp;
+  const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
+  for (int j = ly; j < 32; j += 8) {
+    const long o = (long)(ti * 32 + j) * q.mp + tj * 32 + lx;
+    float v = 0.f;
+    for (int s = 0; s < q.splits; ++s) v += in[s * plane + o];
+    v *= SA / (SX * SX);
+    tile[j][lx] = v;
+    split16(v, A[o], A[plane + o]);
+  }
+  if (ti == tj) return;      // the whole block: it is symmetric by itself
+  __syncthreads();
+  for (int j = ly; j < 32; j += 8) {
+    const long o = (long)(tj * 32 + j) * q.mp + ti * 32 + lx;
+    split16(tile[lx][j], A[o], A[plane + o]);
+  }
+}
+
+// W = a I + b A + c A A, lower tiles, both triangles written
+__global__ __launch_bounds__(256, 2) void ns_poly(const NsArgs p) {
+  extern __shared__ __align__(16) _Float16 lds[];
+  const int i = ns_find(p, blockIdx.x);
+  const NsMat& q = p.mat[i];
+  int ti, tj;
+  tri(blockIdx.x - p.pre[i], ti, tj);
+  const long plane = (long)q.mp * q.mp;
+  const _Float16* A = (const _Float16*)(p.ws + q.off_a);
+  _Float16* Wp = (_Float16*)(p.ws + q.off_a) + 2 * plane;
+  f32x16 acc[2][2];
+  ns_tile<false>(A, plane, q.mp, A, plane, q.mp, ti * NS_TILE, tj * NS_TILE, 0, q.mp, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int c = tj * NS_TILE + (wave & 1) * 64 + b * 32 + (lane & 31);
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f16x4 hi, lo;
+        const int row0 = ti * NS_TILE + (wave >> 1) * 64 + a * 32 + c_row(4 * r4, lane >> 5);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const long o = (long)(row0 + r) * q.mp + c;
+          float v = p.b * ((float)A[o] + (float)A[plane + o]) + (p.c / SA) * acc[a][b][4 * r4 + r];
+          if (row0 + r == c) v += p.a * SA;
+          _Float16 h, l;
+          split16(v, h, l);
+          hi[r] = h;
+          lo[r] = l;
+          Wp[o] = h;
+          Wp[plane + o] = l;
+        }
+        if (ti != tj) {
+          const long o = (long)c * q.mp + row0;
+          *(f16x4*)(Wp + o) = hi;
+          *(f16x4*)(Wp + plane + o) = lo;
+        }
+      }
+    }
+}
+
+// X' = W X; the last step writes the result in its own type and orientation
+__global__ __launch_bounds__(256, 2) void ns_apply(const NsArgs p, int buf, int last) {
+  extern __shared__ __align__(16) _Float16 lds[];
+  const int i = ns_find(p, blockIdx.x);
+  const NsMat& q = p.mat[i];
+  const int id = blockIdx.x - p.pre[i], mt = q.mp / NS_TILE, r0 = id % mt * NS_TILE, c0 = id / mt * NS_TILE;
+  const long plane = (long)q.mp * q.np, planeW = (long)q.mp * q.mp;
+  const _Float16* W = (const _Float16*)(p.ws + q.off_a) + 2 * planeW;
+  const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
+  _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
+  f32x16 acc[2][2];
+  ns_tile<true>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool tall = q.rows > q.cols;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int c = c0 + (wave & 1) * 64 + b * 32 + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5);
+        const float v = acc[a][b][r] * (1.f / SA);
+        if (last) {
+          if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, v * (1.f / SX));
+        } else {
+          const long o = (long)row * q.np + c;
+          split16(v, y[o], y[plane + o]);
+        }
+      }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ small matrices
+// One workgroup of eight waves holds a matrix: X's planes, and A's (W's after it, in the same place), stay in LDS for all
+// steps, so a list of encoder matrices is one launch.  Bound by the chain of barriers: four a step.
+struct NsSmallArgs {
+  float a, b, c, eps;
+  int steps;
+  NsMat mat[NS_MAXMAT];
+};
+
+__host__ __device__ inline int ns_small_splits(int mt) { return mt == 1 ? 8 : mt == 2 ? 2 : 1; }
+inline size_t ns_small_lds(int mp, int np) {
+  const int mt = mp / 32, sp = ns_small_splits(mt);
+  return (size_t)4 * mp * (np + 8) + (size_t)4 * mp * (mp + 8) + (size_t)(sp - 1) * mt * mt * 4096;
+}
+inline bool ns_is_small(int mp, int np) {
+  return mp / 32 <= 4 && (mp / 32) * (np / 32) <= 32 && ns_small_lds(mp, np) <= NS_SMALL_LDS;
+}
+
+__global__ __launch_bounds__(512) void ns_small(const NsSmallArgs p) {
+  extern __shared__ __align__(16) _Float16 lds[];
+  __shared__ double red[8];
+  const NsMat& q = p.mat[blockIdx.x];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5;
+  const int mp = q.mp, np = q.np, ldx = np + 8, lda = mp + 8, mt = mp / 32, nt = np / 32;
+  _Float16 *Xh = lds, *Xl = Xh + mp * ldx, *Ah = Xl + mp * ldx, *Al = Ah + mp * lda;
+  float* part = (float*)(Al + mp * lda);
+  const bool tall = q.rows > q.cols;
+  const int total = q.rows * q.cols;
+  double s = 0.;
+  for (int i = t; i < total; i += 512) {
+    const double v = ns_load(q, i / q.cols, i % q.cols);
+    s = fma(v, v, s);
+  }
+  const float scale = (float)(SX / (sqrt(block_sum64(s, red)) + (double)p.eps));
+  for (int i = t; i < mp * np; i += 512) {        // the source's fast index is the thread's
+    const int fast = tall ? i % mp : i % np, slow = tall ? i / mp : i / np, r = tall ? fast : slow, c = tall ? slow : fast;
+    const float v = r < q.m && c < q.n ? ns_load(q, tall ? c : r, tall ? r : c) * scale : 0.f;
+    split16(v, Xh[r * ldx + c], Xl[r * ldx + c]);
+  }
+  __syncthreads();
+  const int splits = ns_small_splits(mt), units = mt * mt * splits;
+  for (int step = 0; step < p.steps; ++step) {
+    f32x16 acc[4];
+    // A = X X^T: wave takes unit u = (tile, share of the columns)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int u = wave + 8 * j;
+      acc[j] = 0.f;
+      if (u >= units) continue;
+      const int tile = u / splits, sp = u % splits, ti = tile / mt, tj = tile % mt;
+      const int chunks = np / 16, per = (chunks + splits - 1) / splits;
+      for (int k = sp * per; k < min(chunks, (sp + 1) * per); ++k) {
+        const f16x8 ah = frag_k(Xh, ldx, ti * 32, k * 16, lane), al = frag_k(Xl, ldx, ti * 32, k * 16, lane);
+        const f16x8 bh = frag_k(Xh, ldx, tj * 32, k * 16, lane), bl = frag_k(Xl, ldx, tj * 32, k * 16, lane);
+        acc[j] = MFMA16(al, bh, acc[j]);
+        acc[j] = MFMA16(ah, bl, acc[j]);
+        acc[j] = MFMA16(ah, bh, acc[j]);
+      }
+      if (sp > 0) {
+        float* o = part + ((sp - 1) * mt * mt + tile) * 1024 + lane;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[r * 64] = acc[j][r];
+      }
+    }
+    if (splits > 1) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int u = wave + 8 * j;
+      if (u >= units || u % splits) continue;
+      const int tile = u / splits, ti = tile / mt, tj = tile % mt;
+      for (int sp = 1; sp < splits; ++sp) {
+        const float* o = part + ((sp - 1) * mt * mt + tile) * 1024 + lane;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[j][r] += o[r * 64];
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int o = (ti * 32 + c_row(r, h)) * lda + tj * 32 + (lane & 31);
+        split16(acc[j][r] * (SA / (SX * SX)), Ah[o], Al[o]);
+      }
+    }
+    __syncthreads();
+    // W = a I + b A + c A A into A's place
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tile = wave + 8 * j;
+      if (tile >= mt * mt) continue;
+      const int ti = tile / mt, tj = tile % mt;
+      f32x16 sq = 0.f;
+      for (int k = 0; k < mp; k += 16) {
+        const f16x8 ah = frag_k(Ah, lda, ti * 32, k, lane), al = frag_k(Al, lda, ti * 32, k, lane);
+        const f16x8 bh = frag_k(Ah, lda, tj * 32, k, lane), bl = frag_k(Al, lda, tj * 32, k, lane);
+        sq = MFMA16(al, bh, sq);
+        sq = MFMA16(ah, bl, sq);
+        sq = MFMA16(ah, bh, sq);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = ti * 32 + c_row(r, h), c = tj * 32 + (lane & 31);
+        const float av = (float)Ah[row * lda + c] + (float)Al[row * lda + c];
+        acc[j][r] = p.b * av + (p.c / SA) * sq[r] + (row == c ? p.a * SA : 0.f);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tile = wave + 8 * j;
+      if (tile >= mt * mt) continue;
+      const int ti = tile / mt, tj = tile % mt;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int o = (ti * 32 + c_row(r, h)) * lda + tj * 32 + (lane & 31);
+        split16(acc[j][r], Ah[o], Al[o]);
+      }
+    }
+    __syncthreads();
+    // X' = W X, up to four tiles a wave
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int tile = wave + 8 * j;
+      acc[j] = 0.f;
+      if (tile >= mt * nt) continue;
+      const int ti = tile / nt, tj = tile % nt;
+      for (int k = 0; k < mp; k += 16) {
+        const f16x8 ah = frag_kp(Ah, lda, ti * 32, k, lane), al = frag_kp(Al, lda, ti * 32, k, lane);
+        const f16x8 bh = frag_t(Xh, ldx, k, tj * 32, lane), bl = frag_t(Xl, ldx, k, tj * 32, lane);
+        acc[j] = MFMA16(al, bh, acc[j]);
+        acc[j] = MFMA16(ah, bl, acc[j]);
+        acc[j] = MFMA16(ah, bh, acc[j]);
+      }
+    }
+    __syncthreads();
+    const bool last = step + 1 == p.steps;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int tile = wave + 8 * j;
+      if (tile >= mt * nt) continue;
+      const int ti = tile / nt, tj = tile % nt;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = ti * 32 + c_row(r, h), c = tj * 32 + (lane & 31);
+        const float v = acc[j][r] * (1.f / SA);
+        if (!last) split16(v, Xh[row * ldx + c], Xl[row * ldx + c]);
+        else if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, v * (1.f / SX));
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+// Layout of a matrix of the large form in the workspace; returns the bytes used.
+size_t ns_layout(NsMat& q, size_t off) {
+  const auto take = [&](size_t n) { const size_t o = off; off = (off + n + 255) / 256 * 256; return (long)o; };
+  q.off_x = take((size_t)8 * q.mp * q.np);         // two buffers of two planes
+  q.off_a = take((size_t)8 * q.mp * q.mp);         // A and W
+  q.off_p = take((size_t)4 * q.splits * q.mp * q.mp);
+  q.off_s = take((size_t)8 * NS_SUMSQ_BLOCKS);
+  return off;
+}
+
+void ns_dims(NsMat& q, const ctr_ns_mat_t& g, int type) {
+  q = NsMat{};
+  q.src = g.src;
+  q.dst = g.dst;
+  q.ld_src = g.ld_src;
+  q.ld_dst = g.ld_dst;
+  q.rows = g.rows;
+  q.cols = g.cols;
+  q.type = type;
+  q.m = std::min(g.rows, g.cols);
+  q.n = std::max(g.rows, g.cols);
+  q.mp = cdiv(q.m, 32) * 32;
+  q.np = cdiv(q.n, 32) * 32;
+}
+
+bool ns_large_dims(NsMat& q) {
+  if (ns_is_small(q.mp, q.np)) return false;
+  q.mp = cdiv(q.m, NS_TILE) * NS_TILE;
+  q.np = cdiv(q.n, NS_TILE) * NS_TILE;
+  const int nt = q.mp / NS_TILE, tiles = nt * (nt + 1) / 2;
+  q.splits = std::max(1, std::min(512 / tiles, q.np / NS_TILE));
+  return true;
+}
+
+// the largest singular value that X can reach, and W: the polynomial scanned over [0, r] each step
+bool ns_in_range(int steps, double a, double b, double c) {
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+  double r = 1.0;
+  for (int s = 0; s < steps; ++s) {
+    double next = 0., w = 0.;
+    for (int i = 0; i <= 4096; ++i) {
+      const double v = r * i / 4096, v2 = v * v, pv = std::fabs(a + b * v2 + c * v2 * v2);
+      w = std::max(w, pv);
+      next = std::max(next, v * pv);
+    }
+    if (!(w <= 32.) || !(next <= 7.5)) return false;
+    r = next * 1.001;
+  }
+  return true;
+}
+
+// the kernels' LDS beyond 64 KB, once for each device
+bool ns_allow_lds() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load() & bit) return true;
+  const int tile_lds = 8 * PLANE_K * (int)sizeof(_Float16);
+  const auto allow = [](const void* f, int n) {
+    return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n) == hipSuccess;
+  };
+  if (!allow((const void*)ns_gram, tile_lds) || !allow((const void*)ns_poly, tile_lds) ||
+      !allow((const void*)ns_apply, tile_lds) || !allow((const void*)ns_small, NS_SMALL_LDS))
+    return false;
+  done.fetch_or(bit);
+  return true;
+}
+
+}  // namespace
+}  // namespace ctr
+
+using namespace ctr;
+
+extern "C" size_t ctr_newton_schulz_ws_size(const ctr_ns_mat_t* mats, int count) {
+  size_t most = 0, off = 0;
+  int in = 0;
+  for (int i = 0; mats && i < count; ++i) {
+    if (mats[i].rows <= 0 || mats[i].cols <= 0) continue;
+    NsMat q;
+    ns_dims(q, mats[i], 0);
+    if (!ns_large_dims(q)) continue;
+    if (in == NS_MAXMAT) in = 0, off = 0;
+    off = ns_layout(q, off);
+    ++in;
+    most = std::max(most, off);
+  }
+  return most;
+}
+
+extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps, float a, float b, float c, float eps,
+                                 int type, void* ws, size_t ws_bytes, void* stream) {
+  CTR_REQUIRE(count >= 0 && (count == 0 || mats), "matrix list");
+  CTR_REQUIRE(type >= TY_F32 && type <= TY_F16, "type (0 fp32, 1 bf16, 2 fp16)");
+  CTR_REQUIRE(steps >= 1 && steps <= 64, "steps in [1, 64]");
+  CTR_REQUIRE(eps >= 0.f && std::isfinite(eps), "eps");
+  CTR_REQUIRE(ns_in_range(steps, a, b, c), "coefficients: a singular value could pass 7.5, or one of a I + b A + c A^2 32");
+  for (int i = 0; i < count; ++i) {
+    const ctr_ns_mat_t& g = mats[i];
+    CTR_REQUIRE(g.rows >= 0 && g.cols >= 0 && g.rows <= 65536 && g.cols <= 65536, "matrix sides in [0, 65536]");
+    if (g.rows == 0 || g.cols == 0) continue;
+    CTR_REQUIRE(g.src && g.dst, "null matrix");
+    CTR_REQUIRE((g.rows == 1 || g.ld_src >= g.cols) && (g.rows == 1 || g.ld_dst >= g.cols), "row strides");
+  }
+  CTR_REQUIRE(ws_bytes >= ctr_newton_schulz_ws_size(mats, count), "workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  CTR_REQUIRE(ns_allow_lds(), "LDS size attribute");
+
+  NsSmallArgs small = {a, b, c, eps, steps, {}};
+  int ns = 0;
+  size_t small_lds = 0;
+  const auto flush_small = [&] {
+    if (ns) ns_small<<<ns, 512, small_lds, s>>>(small);
+    ns = 0;
+    small_lds = 0;
+  };
+  NsArgs large = {};
+  large.ws = (char*)ws;
+  large.a = a;
+  large.b = b;
+  large.c = c;
+  large.eps = eps;
+  size_t off = 0;
+  const auto prefix = [&](auto blocks) {
+    int n = 0;
+    for (int i = 0; i < large.count; ++i) {
+      large.pre[i] = n;
+      n += blocks(large.mat[i]);
+    }
+    large.pre[large.count] = n;
+    return n;
+  };
+  const auto flush_large = [&] {
+    if (large.count == 0) return;
+    const size_t lds = 8 * PLANE_K * sizeof(_Float16);
+    ns_sumsq<<<dim3(NS_SUMSQ_BLOCKS, large.count), 256, 0, s>>>(large);
+    const int ni = prefix([](const NsMat& q) { return q.mp / 64 * (q.np / 64); });
+    ns_init<<<ni, 256, 0, s>>>(large);
+    for (int k = 0; k < steps; ++k) {
+      const auto tri_n = [](int n) { return n * (n + 1) / 2; };
+      const int ng = prefix([&](const NsMat& q) { return q.splits * tri_n(q.mp / NS_TILE); });
+      ns_gram<<<ng, 256, lds, s>>>(large, k & 1);
+      const int nj = prefix([&](const NsMat& q) { return tri_n(q.mp / 32); });
+      ns_gram_join<<<nj, 256, 0, s>>>(large);
+      const int np = prefix([&](const NsMat& q) { return tri_n(q.mp / NS_TILE); });
+      ns_poly<<<np, 256, lds, s>>>(large);
+      const int na = prefix([](const NsMat& q) { return q.mp / NS_TILE * (q.np / NS_TILE); });
+      ns_apply<<<na, 256, lds, s>>>(large, k & 1, k + 1 == steps);
+    }
+    large.count = 0;
+    off = 0;
+  };
+  for (int i = 0; i < count; ++i) {
+    if (mats[i].rows == 0 || mats[i].cols == 0) continue;
+    NsMat q;
+    ns_dims(q, mats[i], type);
+    if (ns_large_dims(q)) {
+      if (large.count == NS_MAXMAT) flush_large();
+      off = ns_layout(q, off);
+      large.mat[large.count++] = q;
+    } else {
+      if (ns == NS_MAXMAT) flush_small();
+      small_lds = std::max(small_lds, ns_small_lds(q.mp, q.np));
+      small.mat[ns++] = q;
+    }
+  }
+  flush_small();
+  flush_large();
+  return check_launch("newton_schulz");
+}

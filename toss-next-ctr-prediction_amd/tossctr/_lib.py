@@ -50,6 +50,17 @@ class Seg(C.Structure):
     _fields_ = [("src", p), ("dst", p), ("n", C.c_longlong)]
 
 
+class DiffAttn(C.Structure):
+    _fields_ = [("q", p), ("k", p), ("v", p), ("lam", p), ("o", p), ("o2", p), ("stat", p), ("q_lens", p),
+                ("kv_lens", p), ("q_sb", l), ("q_st", l), ("q_sh", l), ("q_sc", l), ("k_sb", l), ("k_ss", l),
+                ("k_sh", l), ("k_sc", l), ("v_sb", l), ("v_ss", l), ("v_sh", l), ("scale", f), ("B", i), ("T", i),
+                ("S", i), ("H", i), ("Hkv", i), ("D", i), ("causal", i), ("type", i)]
+
+
+class NsMat(C.Structure):
+    _fields_ = [("src", p), ("dst", p), ("ld_src", l), ("ld_dst", l), ("rows", i), ("cols", i)]
+
+
 class LazyTab(C.Structure):
     _fields_ = [("p_off", C.c_int64), ("rows", C.c_int64), ("width", C.c_int32), ("key_base", C.c_uint32),
                 ("last", p)]
@@ -196,6 +207,15 @@ SIGS = {
     "ctr_covis_pair_stats": (i, [p, p, p, p, l, p, p, p, p, i, C.c_double, C.c_double, C.c_double, C.c_double, i,
                                  p, p, p, p, p, p, p, p, p, p, z, p]),
     "ctr_covis_row_features": (i, [p, l, p, p, p, p, p, p, i, C.c_double, p, p, p, p, i, p, p]),
+    "ctr_ln_fwd": (i, [p, l, l, i, p, p, f, p, l, p, p, i, i, p]),
+    "ctr_ln_bwd_ws_size": (z, [l, i]),
+    "ctr_ln_bwd": (i, [p, l, p, l, p, p, p, l, i, p, l, p, p, p, z, i, i, p]),
+    "ctr_diffattn_fwd_ws_size": (z, [C.POINTER(DiffAttn)]),
+    "ctr_diffattn_fwd": (i, [C.POINTER(DiffAttn), p, z, p]),
+    "ctr_diffattn_bwd_ws_size": (z, [C.POINTER(DiffAttn)]),
+    "ctr_diffattn_bwd": (i, [C.POINTER(DiffAttn), p, l, l, l, p, p, p, p, p, z, p]),
+    "ctr_newton_schulz_ws_size": (z, [C.POINTER(NsMat), i]),
+    "ctr_newton_schulz": (i, [C.POINTER(NsMat), i, i, f, f, f, f, i, p, z, p]),
 }
 
 _lib = None
