@@ -11,11 +11,15 @@
 // A wave holds 32 rows (keys in the dK / dV kernel) as the COLUMNS of every product on
 // v_mfma_f32_32x32x16: the scores come out transposed, S^T = K Q^T, so a row's softmax statistics live in one lane (and its
 // neighbour 32 away), the probabilities are already the B operand of O^T = V^T P^T, and a rescale is a lane's own
-// factor.  K, V (Q, dO) tiles of 32 rows go through LDS, read once along a row (ds_read_b128) and once down the columns
-// (the LDS transpose read); 16-byte chunks are XORed with the row so that both are free of bank conflicts.
+// factor.  K, V (Q, dO) tiles of 32 rows go to LDS by buffer loads that write it directly, the next tile's under this
+// tile's products, one barrier a tile; rows behind the end are out of the load's range and come as zeros.  A tile is
+// read once along a row (ds_read_b128) and once down the columns (the LDS transpose read); the 16-byte chunks of a row
+// are XORed with the row, in the global address, so that both reads are free of bank conflicts.
 // Softmax in base 2 with one running maximum per map, taken up only when a score passes it by 2^8; statistics,
-// accumulators and dlam's sum are fp32.  Roundings to 16 bits: P and dS as matrix operands (the instruction's
-// type) and the results; fp16's dS is first scaled by a power of two that follows its size.
+// accumulators and dlam's sum are fp32.
+// Roundings to 16 bits.  The forward's P enter the product with V as two 16-bit terms each (the value and what that leaves
+// out): O is a difference, and where the maps agree one rounding of either would be larger than the result's own.  In
+// the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.
 #include <algorithm>
 #include <atomic>
 
@@ -29,16 +33,20 @@ struct DaArgs {
   const void *q, *k, *v, *dout;
   const float* lam;
   void *o, *o2;                  // (B, T, H, 2 D); o2 = P_2 V, kept for the backward (may be null)
-  float* stat;                   // 4 planes of rows: log2 sums of the maps, then delta_1, delta_2
+  float* stat;                   // 2 planes of rows: log2 sums of the maps
   void *dq, *dk, *dv;
-  float* dlrow;                  // per row sum_j P_2 dP
-  float* part;                   // split keys: partial results
+  float* dlam;
+  float* part;                   // forward, split keys: partial results; backward: row statistics (ROWSTAT)
   const int *q_lens, *kv_lens;
   long q_sb, q_st, q_sh, q_sc, k_sb, k_ss, k_sh, k_sc, v_sb, v_ss, v_sh, g_sb, g_st, g_sh;
   long rows;                     // B Hkv R
   float c, scale;                // scale log2(e), scale
-  int B, T, S, H, Hkv, G, R, causal, splits, tiles;
+  int B, T, S, H, Hkv, G, R, causal, splits, tiles, tiles32;
 };
+
+// Row statistics of the backward, written by the dQ kernel for the dK / dV kernel: a tile of 32 packed rows is 8 lines
+// of 32 words, one 1 KB load
+enum { RS_L1, RS_L2, RS_D1, RS_D2, RS_LAM, RS_LIM, RS_DL, RS_LINES = 8 };
 
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
@@ -53,34 +61,81 @@ template <> struct Mfma<_Float16> {
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // C layout of a 32x32 tile: register r of lane l holds row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32
 __device__ __forceinline__ int c_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// A tile of rows of CH 16-byte chunks in LDS.  Chunk c of a row stands at slot(row, c): sixteen consecutive rows' equal
-// chunks, and four consecutive rows' four-chunk groups, cover the 64 banks once.
+// A tile of 32 rows of W elements in LDS, CH = W / 8 chunks of 16 bytes a row: chunk c of a row stands at chunk
+// c ^ turn(row).  Sixteen consecutive rows' equal chunks, and four consecutive rows' four-chunk groups, then cover the
+// 64 banks once.
 template <int CH>
-__device__ __forceinline__ int slot(int row, int c) {
-  if constexpr (CH >= 16) return row * CH + (c ^ (((row & 3) << 2) | ((row >> 2) & 3)));
-  else return row * CH + (c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)));
+__device__ __forceinline__ int turn(int row) {
+  if constexpr (CH >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else if constexpr (CH == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else return (row >> 2) & 3;
 }
 // 32 rows x 16 k, k contiguous along a row: lane l has row l % 32, k = 16 kk + 8 (l / 32) + 0..7
-template <typename T, int CH>
+template <typename T, int W>
 __device__ __forceinline__ typename Vec<T>::v8 frag_row(const T* s, int kk, int lane) {
-  return *(const typename Vec<T>::v8*)(s + slot<CH>(lane & 31, 2 * kk + (lane >> 5)) * 8);
+  const int row = lane & 31;
+  return *(const typename Vec<T>::v8*)(s + row * W + ((2 * kk + (lane >> 5)) ^ turn<W / 8>(row)) * 8);
 }
-// 16 rows (from r0) as k x 32 columns (from c0): lane l has column l % 32 and the rows 4 (l / 32) + 0..3, 8 + 4 (l / 32)
-// + 0..3 -- the order in which a C tile's registers 8 i .. 8 i + 7 hold the rows of its i-th half
-template <typename T, int CH>
-__device__ __forceinline__ typename Vec<T>::v8 frag_col(const T* s, int r0, int c0, int lane) {
-  const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2), c = c0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-  auto p = (__attribute__((address_space(3))) s16x4*)(s + slot<CH>(row, c >> 3) * 8 + (c & 4));
-  auto p8 = (__attribute__((address_space(3))) s16x4*)(s + slot<CH>(row + 8, c >> 3) * 8 + (c & 4));
-  const auto u = __builtin_bit_cast(typename Vec<T>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
-  const auto w = __builtin_bit_cast(typename Vec<T>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p8));
-  return __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
+// Transposed reads.  The 32 rows of a tile as k x 32 columns: for the first and second 16 rows, lane l gets of column l % 32
+// the rows 4 (l / 32) + 0..3 and 8 + 4 (l / 32) + 0..3 -- the order in which a C tile's registers 8 i .. 8 i + 7 hold the
+// rows of its i-th half.  A group of 16 lanes takes 4 rows of 16 columns: lane i of it the address of row i / 4,
+// columns 4 (i % 4), and it gets column i.  `col_base` is the lane's address for the columns from 0; columns 32 j on are
+// at col_base ^ (j << 6), since a panel's chunks are XORed and its rows start at multiples of their power-of-two size; 8 rows
+// on the turn differs by 2, 16 rows on it is the same.
+template <typename T, int W>
+__device__ __forceinline__ uint32_t col_base(const T* s, int lane) {
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)(s + row * W + ((c >> 3) ^ turn<W / 8>(row)) * 8 + (c & 4));
 }
-// registers 8 i .. 8 i + 7 of a C tile as an operand
+// Two column groups, 4 fragments.  The reads and their wait are one block: the compiler, which sees no address in the
+// transpose read, would wait for the next tile's loads before it.
+template <typename T, int W>
+__device__ __forceinline__ void frag_col2(uint32_t base, int j0, int j1, typename Vec<T>::v8 (&f)[2][2]) {
+  typedef typename Vec<T>::v4 v4;
+  const uint32_t p0 = base ^ (j0 << 6), p1 = base ^ (j1 << 6), q0 = (p0 + 16 * W) ^ 32, q1 = (p1 + 16 * W) ^ 32;
+  v4 a, b, c, d, e, g, h, i;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\t"
+      "ds_read_b64_tr_b16 %1, %9\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\t"
+      "ds_read_b64_tr_b16 %5, %11\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(g), "=&v"(h), "=&v"(i)
+      : "v"(p0), "v"(q0), "v"(p1), "v"(q1), "n"(32 * W)
+      : "memory");
+  f[0][0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  f[0][1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+  f[1][0] = __builtin_shufflevector(e, g, 0, 1, 2, 3, 4, 5, 6, 7);
+  f[1][1] = __builtin_shufflevector(h, i, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// one column group
+template <typename T, int W>
+__device__ __forceinline__ void frag_col1(uint32_t base, typename Vec<T>::v8 (&f)[2]) {
+  typedef typename Vec<T>::v4 v4;
+  const uint32_t q0 = (base + 16 * W) ^ 32;
+  v4 a, b, c, d;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\t"
+      "ds_read_b64_tr_b16 %1, %5\n\t"
+      "ds_read_b64_tr_b16 %2, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+      : "v"(base), "v"(q0), "n"(32 * W)
+      : "memory");
+  f[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  f[1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// registers 8 i .. 8 i + 7 of a C tile as an operand, and what the rounding left out
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::v8 pack(const f32x16& v, int i) {
   f32x8 o;
@@ -88,19 +143,85 @@ __device__ __forceinline__ typename Vec<T>::v8 pack(const f32x16& v, int i) {
   for (int j = 0; j < 8; ++j) o[j] = v[8 * i + j];
   return __builtin_convertvector(o, typename Vec<T>::v8);
 }
-
-// 32 rows to LDS: NT threads, row r from src + row_off(r), its second half at `half` elements more; rows from `valid` on
-// are zeros (what stands behind the end of a cache is not read)
-template <typename T, int CH, int NT, typename F>
-__device__ __forceinline__ void load_tile(T* dst, int valid, long half, F row_ptr) {
-  typedef typename Vec<T>::v8 v8;
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::v8 pack_rest(const f32x16& v, typename Vec<T>::v8 hi, int i) {
+  f32x8 o;
+  if constexpr (__is_same(T, __bf16)) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 w = __builtin_bit_cast(u32x4, hi);
 #pragma unroll
-  for (int j = 0; j < (32 * CH + NT - 1) / NT; ++j) {
-    const int i = threadIdx.x + j * NT, r = i / CH, c = i % CH;
-    if ((32 * CH) % NT && i >= 32 * CH) break;
-    v8 x = {};
-    if (r < valid) x = *(const v8*)(row_ptr(r) + (c < CH / 2 ? c * 8 : half + (c - CH / 2) * 8));
-    *(v8*)(dst + slot<CH>(r, c) * 8) = x;
+    for (int j = 0; j < 4; ++j) {
+      o[2 * j] = v[8 * i + 2 * j] - __builtin_bit_cast(float, w[j] << 16);
+      o[2 * j + 1] = v[8 * i + 2 * j + 1] - __builtin_bit_cast(float, w[j] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = v[8 * i + j] - (float)hi[j];
+  }
+  return __builtin_convertvector(o, typename Vec<T>::v8);
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+// Direct loads of a tile of 32 rows to LDS: two panels of width D (the maps) and one of 2 D (values, or dO), as four
+// roles dealt over the waves: panel 0, panel 1, the upper and the lower 16 rows of panel 2.  Each role is PER loads of
+// 64 lanes x 16 bytes, whose LDS places are consecutive.
+template <typename T, int D, int NW>
+struct Stage {
+  static constexpr int PER = D / 16, TILE = 32 * 4 * D, ROLES = 4 / NW;      // TILE: elements of the three panels
+  int row[ROLES], byte[ROLES][PER];      // the lane's row for load 0 of its roles, and its byte in the row for each load
+  static __device__ __forceinline__ int panel_offset(int role) { return role < 2 ? role * 32 * D : 64 * D + (role - 2) * 32 * D; }
+  static __device__ __forceinline__ int step(int role) { return role < 2 ? 512 / D : 256 / D; }      // rows from load to load
+  __device__ __forceinline__ Stage(int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < ROLES; ++i) {
+      const int role = i * NW + wave;
+      const bool map = role < 2;
+      row[i] = map ? lane / (D / 8) : lane / (D / 4) + (role - 2) * 16;
+      const int c = map ? lane % (D / 8) : lane % (D / 4);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int r = row[i] + j * step(role);
+        byte[i][j] = (c ^ (map ? turn<D / 8>(r) : turn<D / 4>(r))) * 16;
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t open_range(const void* p) { return buf_rsrc(p, 0x7ffffff0u); }
+
+// every wave's loads of the next tile are in LDS and every wave is done with the last one
+__device__ __forceinline__ void tile_ready() {
+  asm volatile("" ::: "memory");           // the builtins order nothing for the compiler
+  __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// keys [kb, kb + 32) of K_1, K_2, V to one buffer; rows from `valid` on come as zeros
+template <typename T, int D, int NW>
+__device__ __forceinline__ void stage_keys(const DaArgs& a, const Stage<T, D, NW>& p, const T* kp, const T* vp, int kb, int valid,
+                                           T* buf, int wave) {
+  typedef Stage<T, D, NW> St;
+#pragma unroll
+  for (int i = 0; i < St::ROLES; ++i) {
+    const int role = i * NW + wave;
+    const T* base = role < 2 ? kp + (long)kb * a.k_ss + (role ? a.k_sc : 0) : vp + (long)kb * a.v_ss;
+    const int stride = (int)((role < 2 ? a.k_ss : a.v_ss) * sizeof(T)), step = St::step(role);
+    const auto rs = open_range(base);
+    T* dst = buf + St::panel_offset(role);
+    int row = p.row[i], off = row * stride;
+    if (valid >= 32) {
+#pragma unroll
+      for (int j = 0; j < St::PER; ++j, off += step * stride) dma16(rs, dst + j * 512, off + p.byte[i][j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < St::PER; ++j, off += step * stride, row += step)
+        dma16(rs, dst + j * 512, row < valid ? off + p.byte[i][j] : BUF_OOB);
+    }
   }
 }
 
@@ -120,179 +241,219 @@ struct Seq {
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_fwd(const DaArgs a) {
-  constexpr int CH = D / 4, DV = 2 * D, NT = 64 * NW, KQ = D / 16, NO = DV / 32;
+// A pair of waves owns 32 rows, one of them each map: nothing but the value tile's reads is done twice, a wave's
+// accumulators are half as many, and three (D = 64) or two (D = 128) waves share a SIMD, so that one's exponentials run
+// under another's products.  RG pairs a workgroup.
+// Workgroups: (batch, key head) fastest, so that the eight XCDs, which take workgroups in turn, each keep few heads'
+// keys in their L2; then the splits, then the row tiles, the causally longest first.
+template <typename T, int D, int RG>
+__global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da_fwd(const DaArgs a) {
+  constexpr int DV = 2 * D, KQ = D / 16, NO = DV / 32, NW = 2 * RG, TILE = Stage<T, D, NW>::TILE;
+  static_assert(RG * DV * 32 * sizeof(float) <= 2 * TILE * sizeof(T), "the maps meet in the tiles' place");
   typedef typename Vec<T>::v8 v8;
-  __shared__ __align__(16) T ks[32 * DV], vs[32 * DV];
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  __shared__ __align__(1024) T tiles[2][TILE];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nbh = a.B * a.Hkv;
+  const Stage<T, D, NW> plan(wave, lane);
+  const int map = wave & 1, pair = wave >> 1;
   int id = blockIdx.x;
-  const int tile = id % a.tiles;
-  id /= a.tiles;
-  const int bh = id % (a.B * a.Hkv), sp = id / (a.B * a.Hkv);
+  const int bh = id % nbh;
+  id /= nbh;
+  const int sp = id % a.splits, tile = a.tiles - 1 - id / a.splits;
   const Seq s(a, bh);
-  const int row = tile * 32 * NW + wave * 32 + (lane & 31), rr = min(row, a.R - 1), t = rr / a.G, head = s.hk * a.G + rr - t * a.G;
+  const int row = tile * 32 * RG + pair * 32 + (lane & 31), rr = min(row, a.R - 1), t = rr / a.G, head = s.hk * a.G + rr - t * a.G;
   const int lim = s.limit(a, t);
   // the keys of the block: those its last row sees, and of them this split's share
-  const int t_last = min((min(tile * 32 * NW + 32 * NW, a.R) - 1) / a.G, s.ql - 1);
+  const int t_last = min((min(tile * 32 * RG + 32 * RG, a.R) - 1) / a.G, s.ql - 1);
   int k0 = 0, k1 = t_last < 0 ? 0 : s.limit(a, t_last);
   if (a.splits > 1) {
     const int per = (((k1 + a.splits - 1) / a.splits) + 31) / 32 * 32;
     k0 = min(k1, sp * per);
     k1 = min(k1, k0 + per);
   }
-  const T* qp = (const T*)a.q + s.b * a.q_sb + t * a.q_st + head * a.q_sh;
-  v8 qf[2][KQ];
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int k = 0; k < KQ; ++k) qf[c][k] = *(const v8*)(qp + c * a.q_sc + 16 * k + 8 * h);
   const T* kp = (const T*)a.k + s.b * a.k_sb + s.hk * a.k_sh;
   const T* vp = (const T*)a.v + s.b * a.v_sb + s.hk * a.v_sh;
-  f32x16 o[2][NO];
+  if (k0 < k1) stage_keys<T, D, NW>(a, plan, kp, vp, k0, k1 - k0, tiles[0], wave);
+  const T* qp = (const T*)a.q + s.b * a.q_sb + t * a.q_st + head * a.q_sh + map * a.q_sc;
+  v8 qf[KQ];
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+  for (int k = 0; k < KQ; ++k) qf[k] = *(const v8*)(qp + 16 * k + 8 * h);
+  f32x16 o[NO];
 #pragma unroll
-    for (int j = 0; j < NO; ++j) o[c][j] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  for (int kb = k0; kb < k1; kb += 32) {
-    __syncthreads();
-    load_tile<T, CH, NT>(ks, min(32, k1 - kb), a.k_sc, [&](int r) { return kp + (long)(kb + r) * a.k_ss; });
-    load_tile<T, CH, NT>(vs, min(32, k1 - kb), D, [&](int r) { return vp + (long)(kb + r) * a.v_ss; });
-    __syncthreads();
-    f32x16 sc[2];
+  for (int j = 0; j < NO; ++j) o[j] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const uint32_t vcol = col_base<T, DV>(tiles[0] + 64 * D, lane);
+  int cur = 0;
+  for (int kb = k0; kb < k1; kb += 32, cur ^= 1) {
+    tile_ready();
+    if (kb + 32 < k1) stage_keys<T, D, NW>(a, plan, kp, vp, kb + 32, k1 - kb - 32, tiles[cur ^ 1], wave);
+    const T* ks = tiles[cur] + map * 32 * D;
+    f32x16 sc = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      sc[c] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, CH>(ks, c * KQ + k, lane), qf[c][k], sc[c]);
-    }
+    for (int k = 0; k < KQ; ++k) sc = Mfma<T>::run(frag_row<T, D>(ks, k, lane), qf[k], sc);
     const int end = min(lim, k1) - kb;
     if (__any(end < 32)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const bool seen = c_row(r, h) < end;
-        sc[0][r] = seen ? sc[0][r] : -INFINITY;
-        sc[1][r] = seen ? sc[1][r] : -INFINITY;
-      }
+      for (int r = 0; r < 16; ++r) sc[r] = c_row(r, h) < end ? sc[r] : -INFINITY;
     }
-    v8 pf[2][2];
+    float top = sc[0];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float top = sc[c][0];
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any((top - m) * a.c > 8.f)) {        // also the first keys, from -inf (-inf - -inf is NaN: no)
+      const float mn = fmaxf(m, top), f = m == mn ? 1.f : exp2f((m - mn) * a.c);
+      l *= f;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[c][r]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any((top - m[c]) * a.c > 8.f)) {        // also the first keys: from -inf (equal -inf gives NaN: no)
-        const float mn = fmaxf(m[c], top), f = m[c] == mn ? 1.f : exp2f((m[c] - mn) * a.c);
-        l[c] *= f;
-#pragma unroll
-        for (int j = 0; j < NO; ++j) o[c][j] *= f;
-        m[c] = mn;
-      }
-      const float base = m[c] == -INFINITY ? 0.f : m[c] * a.c;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        sc[c][r] = __builtin_amdgcn_exp2f(fmaf(sc[c][r], a.c, -base));
-        l[c] += sc[c][r];
-      }
-      pf[c][0] = pack<T>(sc[c], 0);
-      pf[c][1] = pack<T>(sc[c], 1);
+      for (int j = 0; j < NO; ++j) o[j] *= f;
+      m = mn;
     }
+    const float base = m == -INFINITY ? 0.f : m * a.c;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], a.c, -base));
+      l += sc[r];
+    }
+    v8 pf[2], pr[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      pf[i] = pack<T>(sc, i);
+      pr[i] = pack_rest<T>(sc, pf[i], i);
+    }
+    const uint32_t vc = vcol + cur * TILE * sizeof(T);
+#pragma unroll
+    for (int j = 0; j < NO; j += 2) {
+      v8 vf[2][2];
+      frag_col2<T, DV>(vc, j, j + 1, vf);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          o[j + e] = Mfma<T>::run(vf[e][i], pr[i], o[j + e]);
+          o[j + e] = Mfma<T>::run(vf[e][i], pf[i], o[j + e]);
+        }
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  const long n = (long)bh * a.R + row;
+  if (a.splits > 1) {
+    if (row >= a.R) return;
+    float* p = a.part + ((long)sp * a.rows + n) * (2 * DV + 4);
 #pragma unroll
     for (int j = 0; j < NO; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const v8 vf = frag_col<T, CH>(vs, 16 * i, 32 * j, lane);
-        o[0][j] = Mfma<T>::run(vf, pf[0][i], o[0][j]);
-        o[1][j] = Mfma<T>::run(vf, pf[1][i], o[1][j]);
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = o[j][4 * r4 + r];
+        *(f32x4*)(p + map * DV + 32 * j + 8 * r4 + 4 * h) = x;
       }
-  }
-#pragma unroll
-  for (int c = 0; c < 2; ++c) l[c] += __shfl_xor(l[c], 32, 64);
-  if (row >= a.R) return;
-  const long n = (long)bh * a.R + row;
-  if (a.splits > 1) {
-    float* p = a.part + ((long)sp * a.rows + n) * (2 * DV + 4);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-      for (int j = 0; j < NO; ++j)
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          f32x4 x;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = o[c][j][4 * r4 + r];
-          *(f32x4*)(p + c * DV + 32 * j + 8 * r4 + 4 * h) = x;
-        }
-      if (h == 0) {
-        p[2 * DV + 2 * c] = m[c];
-        p[2 * DV + 2 * c + 1] = l[c];
-      }
+    if (h == 0) {
+      p[2 * DV + 2 * map] = m;
+      p[2 * DV + 2 * map + 1] = l;
     }
     return;
   }
-  const float lam = a.lam[head];
-  const float i1 = l[0] > 0.f ? 1.f / l[0] : (l[0] == 0.f ? 0.f : l[0]), i2 = l[1] > 0.f ? 1.f / l[1] : (l[1] == 0.f ? 0.f : l[1]);
-  const long out = ((long)(s.b * a.T + t) * a.H + head) * DV;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (a.stat && h == 0 && row < a.R)           // a row that sees nothing: +inf, so that its P comes out 0
+    a.stat[map * a.rows + n] = l == 0.f ? INFINITY : fmaf(m, a.c, log2f(l));
+  // the second map's part goes through LDS to the first map's wave (each path by itself: a value that both change would be
+  // copied register by register)
+  float* meet = (float*)&tiles[0][0] + pair * DV * 32 + (lane & 31);
+  const long at = ((long)(s.b * a.T + t) * a.H + head) * DV;
+  __syncthreads();
+  if (map) {
 #pragma unroll
-  for (int j = 0; j < NO; ++j)
+    for (int j = 0; j < NO; ++j)
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      typename Vec<T>::v4 x, y;
+      for (int r = 0; r < 16; ++r) meet[(32 * j + c_row(r, h)) * 32] = o[j][r] * inv;
+  }
+  __syncthreads();
+  if (row >= a.R) return;
+  const auto put = [&](T* out, int j, int r4, const f32x4& v) {
+    *(typename Vec<T>::v4*)(out + 32 * j + 8 * r4 + 4 * h) = __builtin_convertvector(v, typename Vec<T>::v4);
+  };
+  if (map) {
+    if (!a.o2) return;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float u = o[0][j][4 * r4 + r] * i1, w = o[1][j][4 * r4 + r] * i2;
-        x[r] = (T)(u - lam * w);
-        y[r] = (T)w;
+    for (int j = 0; j < NO; ++j)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = o[j][4 * r4 + r] * inv;
+        put((T*)a.o2 + at, j, r4, x);
       }
-      const long p = out + 32 * j + 8 * r4 + 4 * h;
-      *(typename Vec<T>::v4*)((T*)a.o + p) = x;
-      if (a.o2) *(typename Vec<T>::v4*)((T*)a.o2 + p) = y;
-    }
-  if (a.stat && h == 0) {          // a row that sees nothing: +inf, so that its P comes out 0
+  } else {
+    const float lam = a.lam[head];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) a.stat[c * a.rows + n] = l[c] == 0.f ? INFINITY : fmaf(m[c], a.c, log2f(l[c]));
+    for (int j = 0; j < NO; ++j) {
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = o[j][4 * r4 + r] * inv - lam * meet[(32 * j + c_row(4 * r4 + r, h)) * 32];
+        put((T*)a.o + at, j, r4, x);
+      }
+      __builtin_amdgcn_sched_barrier(0);       // one tile's reads at a time: the accumulators fill the registers
+    }
   }
 }
 
-// joins the splits of a row: a wave per row, lane = value columns
+// joins the splits of a row: a workgroup takes 32 value columns of it, eight threads a column the splits in turn
 template <typename T, int D>
-__global__ __launch_bounds__(64) void da_join(const DaArgs a) {
-  constexpr int DV = 2 * D, PER = DV / 64;
+__global__ __launch_bounds__(256) void da_join(const DaArgs a) {
+  constexpr int DV = 2 * D;
+  __shared__ float sh[2][8][32], red[4][8];
   const long n = blockIdx.x;
   const int bh = (int)(n / a.R), r = (int)(n - (long)bh * a.R), b = bh / a.Hkv, hk = bh - b * a.Hkv, t = r / a.G,
-            head = hk * a.G + r - t * a.G, lane = threadIdx.x;
+            head = hk * a.G + r - t * a.G, col = threadIdx.x & 31, grp = threadIdx.x >> 5, c0 = blockIdx.y * 32 + col;
   const float* p = a.part + n * (2 * DV + 4);
   const long step = a.rows * (2 * DV + 4);
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2][PER];
-  for (int s = 0; s < a.splits; ++s)
+  float m[2] = {-INFINITY, -INFINITY};
+  for (int s = threadIdx.x; s < a.splits; s += 256) {
+    m[0] = fmaxf(m[0], p[s * step + 2 * DV]);
+    m[1] = fmaxf(m[1], p[s * step + 2 * DV + 2]);
+  }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) m[c] = fmaxf(m[c], p[s * step + 2 * DV + 2 * c]);
+  for (int c = 0; c < 2; ++c) {
+    m[c] = wave_max(m[c]);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][c] = m[c];
+  }
+  __syncthreads();
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int j = 0; j < PER; ++j) o[c][j] = 0.f;
-  for (int s = 0; s < a.splits; ++s)
+  for (int c = 0; c < 2; ++c) m[c] = fmaxf(fmaxf(red[0][c], red[1][c]), fmaxf(red[2][c], red[3][c]));
+  float l[2] = {0.f, 0.f}, o[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int s = grp; s < a.splits; s += 8)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const float ms = p[s * step + 2 * DV + 2 * c];
       const float f = ms == -INFINITY ? 0.f : ms == m[c] ? 1.f : exp2f((ms - m[c]) * a.c);
       l[c] = fmaf(p[s * step + 2 * DV + 2 * c + 1], f, l[c]);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) o[c][j] = fmaf(p[s * step + c * DV + lane * PER + j], f, o[c][j]);
+      o[c] = fmaf(p[s * step + c * DV + c0], f, o[c]);
     }
-  const float lam = a.lam[head], i1 = l[0] == 0.f ? 0.f : 1.f / l[0], i2 = l[1] == 0.f ? 0.f : 1.f / l[1];
-  const long out = ((long)(b * a.T + t) * a.H + head) * DV + lane * PER;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const float w = o[1][j] * i2;
-    ((T*)a.o)[out + j] = (T)(o[0][j] * i1 - lam * w);
-    if (a.o2) ((T*)a.o2)[out + j] = (T)w;
+  for (int c = 0; c < 2; ++c) {
+    __syncthreads();
+    sh[0][grp][col] = l[c];
+    sh[1][grp][col] = o[c];
+    __syncthreads();
+    if (grp == 0) {
+      l[c] = o[c] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        l[c] += sh[0][g][col];
+        o[c] += sh[1][g][col];
+      }
+    }
   }
-  if (a.stat && lane < 2) {
-    const float ll = lane ? l[1] : l[0], mm = lane ? m[1] : m[0];
-    a.stat[lane * a.rows + n] = ll == 0.f ? INFINITY : fmaf(mm, a.c, log2f(ll));
+  if (grp) return;
+  const float w = l[1] == 0.f ? 0.f : o[1] / l[1];
+  const long out = ((long)(b * a.T + t) * a.H + head) * DV + c0;
+  ((T*)a.o)[out] = (T)((l[0] == 0.f ? 0.f : o[0] / l[0]) - a.lam[head] * w);
+  if (a.o2) ((T*)a.o2)[out] = (T)w;
+  if (a.stat && blockIdx.y == 0 && col < 2) {
+    const float ll = col ? l[1] : l[0], mm = col ? m[1] : m[0];
+    a.stat[col * a.rows + n] = ll == 0.f ? INFINITY : fmaf(mm, a.c, log2f(ll));
   }
 }
 
@@ -301,11 +462,12 @@ __global__ __launch_bounds__(64) void da_join(const DaArgs a) {
 // with the accumulators, when a tile would pass 2^15 (bf16 has fp32's range: always 1)
 template <typename T>
 struct DsScale {
+  static constexpr bool ON = __is_same(T, _Float16);
   float f;
-  __device__ __forceinline__ DsScale() : f(sizeof(T) == 2 && __is_same(T, _Float16) ? 0x1p100f : 1.f) {}
+  __device__ __forceinline__ DsScale() : f(ON ? 0x1p100f : 1.f) {}
   // returns the accumulators' factor (1: nothing to do)
   __device__ __forceinline__ float fit(const f32x16& x, const f32x16& y) {
-    if constexpr (!__is_same(T, _Float16)) return 1.f;
+    if constexpr (!ON) return 1.f;
     float top = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(fabsf(x[r]), fabsf(y[r])));
@@ -320,19 +482,45 @@ struct DsScale {
   }
 };
 
-// dQ: a wave owns 32 rows, walks the keys; also delta_c for the dK / dV kernel and each row's sum of P_2 dP
+// acc[j] += (columns 32 j .. of a panel of width W)^T x
+template <typename T, int W, int N>
+__device__ __forceinline__ void add_cols(uint32_t base, const typename Vec<T>::v8 (&x)[2], f32x16 (&acc)[N]) {
+  static_assert(N == W / 32, "panel");
+  if constexpr (N == 1) {
+    typename Vec<T>::v8 f[2];
+    frag_col1<T, W>(base, f);
+    acc[0] = Mfma<T>::run(f[0], x[0], acc[0]);
+    acc[0] = Mfma<T>::run(f[1], x[1], acc[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      typename Vec<T>::v8 f[2][2];
+      frag_col2<T, W>(base, j, j + 1, f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) acc[j + e] = Mfma<T>::run(f[e][i], x[i], acc[j + e]);
+    }
+  }
+}
+
+// dQ: a wave owns 32 rows, walks the keys; also the rows' statistics for the dK / dV kernel
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaArgs a) {
-  constexpr int CH = D / 4, DV = 2 * D, NT = 64 * NW, KQ = D / 16, KV = DV / 16, NQ = D / 32;
+  constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, TILE = Stage<T, D, NW>::TILE;
   typedef typename Vec<T>::v8 v8;
-  __shared__ __align__(16) T ks[32 * DV], vs[32 * DV];
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-  const int tile = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles;
+  __shared__ __align__(1024) T tiles[2][TILE];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nbh = a.B * a.Hkv;
+  const Stage<T, D, NW> plan(wave, lane);
+  const int bh = blockIdx.x % nbh, tile = a.tiles - 1 - blockIdx.x / nbh;
   const Seq s(a, bh);
   const int row = tile * 32 * NW + wave * 32 + (lane & 31), rr = min(row, a.R - 1), t = rr / a.G, head = s.hk * a.G + rr - t * a.G;
   const int lim = s.limit(a, t);
   const int t_last = min((min(tile * 32 * NW + 32 * NW, a.R) - 1) / a.G, s.ql - 1);
   const int k1 = t_last < 0 ? 0 : s.limit(a, t_last);
+  const T* kp = (const T*)a.k + s.b * a.k_sb + s.hk * a.k_sh;
+  const T* vp = (const T*)a.v + s.b * a.v_sb + s.hk * a.v_sh;
+  if (0 < k1) stage_keys<T, D, NW>(a, plan, kp, vp, 0, k1, tiles[0], wave);
   const T* qp = (const T*)a.q + s.b * a.q_sb + t * a.q_st + head * a.q_sh;
   const T* gp = (const T*)a.dout + s.b * a.g_sb + t * a.g_st + head * a.g_sh;
   const long orow = ((long)(s.b * a.T + t) * a.H + head) * DV, n = (long)bh * a.R + rr;
@@ -358,12 +546,6 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
   d1 = fmaf(lam, d2, d1);           // O_1 = O + lam O_2
   if (lim == 0) d1 = d2 = 0.f;      // a row that sees nothing gives nothing, whatever its dO holds
   const float l1 = a.stat[n], l2 = a.stat[a.rows + n];
-  if (row < a.R && h == 0) {
-    a.stat[2 * a.rows + n] = d1;
-    a.stat[3 * a.rows + n] = d2;
-  }
-  const T* kp = (const T*)a.k + s.b * a.k_sb + s.hk * a.k_sh;
-  const T* vp = (const T*)a.v + s.b * a.v_sb + s.hk * a.v_sh;
   f32x16 dq[2][NQ];
 #pragma unroll
   for (int c = 0; c < 2; ++c)
@@ -371,30 +553,42 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
     for (int j = 0; j < NQ; ++j) dq[c][j] = 0.f;
   float dl = 0.f;
   DsScale<T> fit;
-  for (int kb = 0; kb < k1; kb += 32) {
-    __syncthreads();
-    load_tile<T, CH, NT>(ks, min(32, k1 - kb), a.k_sc, [&](int r) { return kp + (long)(kb + r) * a.k_ss; });
-    load_tile<T, CH, NT>(vs, min(32, k1 - kb), D, [&](int r) { return vp + (long)(kb + r) * a.v_ss; });
-    __syncthreads();
+  const uint32_t kcol = col_base<T, D>(tiles[0], lane);
+  int cur = 0;
+  for (int kb = 0; kb < k1; kb += 32, cur ^= 1) {
+    tile_ready();
+    if (kb + 32 < k1) stage_keys<T, D, NW>(a, plan, kp, vp, kb + 32, k1 - kb - 32, tiles[cur ^ 1], wave);
+    const T* ks = tiles[cur];
+    const T* vs = ks + 64 * D;
     f32x16 sc[2], dp = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       sc[c] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, CH>(ks, c * KQ + k, lane), qf[c][k], sc[c]);
+      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, D>(ks + c * 32 * D, k, lane), qf[c][k], sc[c]);
     }
 #pragma unroll
-    for (int k = 0; k < KV; ++k) dp = Mfma<T>::run(frag_row<T, CH>(vs, k, lane), gf[k], dp);
+    for (int k = 0; k < KV; ++k) dp = Mfma<T>::run(frag_row<T, DV>(vs, k, lane), gf[k], dp);
     const int end = lim - kb;
     const bool edge = __any(end < 32);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const bool seen = !edge || c_row(r, h) < end;
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[0][r], a.c, -l1)), p2 = __builtin_amdgcn_exp2f(fmaf(sc[1][r], a.c, -l2));
-      sc[0][r] = seen ? p1 * (dp[r] - d1) : 0.f;
-      sc[1][r] = seen ? p2 * (dp[r] - d2) : 0.f;
-      dl += seen ? p2 * dp[r] : 0.f;
+      float p1 = __builtin_amdgcn_exp2f(fmaf(sc[0][r], a.c, -l1)), p2 = __builtin_amdgcn_exp2f(fmaf(sc[1][r], a.c, -l2));
+      sc[0][r] = p1 * (dp[r] - d1);
+      sc[1][r] = p2 * (dp[r] - d2);
+      dp[r] *= p2;
     }
+    if (edge) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool seen = c_row(r, h) < end;
+        sc[0][r] = seen ? sc[0][r] : 0.f;
+        sc[1][r] = seen ? sc[1][r] : 0.f;
+        dp[r] = seen ? dp[r] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dl += dp[r];
     const float down = fit.fit(sc[0], sc[1]);
     if (down != 1.f) {
 #pragma unroll
@@ -402,22 +596,28 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
 #pragma unroll
         for (int j = 0; j < NQ; ++j) dq[c][j] *= down;
     }
-    if constexpr (__is_same(T, _Float16)) {
+    if constexpr (DsScale<T>::ON) {
       sc[0] *= fit.f;
       sc[1] *= fit.f;
     }
+    const v8 df[2][2] = {{pack<T>(sc[0], 0), pack<T>(sc[0], 1)}, {pack<T>(sc[1], 0), pack<T>(sc[1], 1)}};
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const v8 df = pack<T>(sc[c], i);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) dq[c][j] = Mfma<T>::run(frag_col<T, CH>(ks, 16 * i, c * D + 32 * j, lane), df, dq[c][j]);
-      }
+    for (int c = 0; c < 2; ++c) add_cols<T, D>(kcol + (cur * TILE + c * 32 * D) * sizeof(T), df[c], dq[c]);
   }
   dl += __shfl_xor(dl, 32, 64);
+  const int t32 = tile * NW + wave;
+  if (h == 0 && t32 < a.tiles32) {
+    float* rs = a.part + ((long)bh * a.tiles32 + t32) * (RS_LINES * 32) + lane;
+    const bool on = row < a.R;
+    rs[32 * RS_L1] = on && lim ? l1 : INFINITY;
+    rs[32 * RS_L2] = on && lim ? l2 : INFINITY;
+    rs[32 * RS_D1] = on ? d1 : 0.f;
+    rs[32 * RS_D2] = on ? d2 : 0.f;
+    rs[32 * RS_LAM] = on ? lam : 0.f;
+    rs[32 * RS_LIM] = __builtin_bit_cast(float, on ? lim : 0);
+    rs[32 * RS_DL] = on ? dl : 0.f;
+  }
   if (row >= a.R) return;
-  if (h == 0) a.dlrow[n] = dl;
   T* out = (T*)a.dq + ((long)(s.b * a.T + t) * a.H + head) * DV;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -434,88 +634,146 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
   }
 }
 
-// dK and dV: a wave owns 32 keys, walks the rows that see them
+// dlam of a head: minus the sum over its rows of sum_j P_2 dP, in fp64, in a fixed order
+__device__ __forceinline__ void head_dlam(const DaArgs& a, int head) {
+  __shared__ double red[16];
+  const int hk = head / a.G, g = head - hk * a.G;
+  double v = 0.;
+  const long total = (long)a.B * a.T;
+  for (long i = threadIdx.x; i < total; i += blockDim.x) {
+    const long b = i / a.T, r = (i - b * a.T) * a.G + g;
+    v += a.part[((b * a.Hkv + hk) * a.tiles32 + (r >> 5)) * (RS_LINES * 32) + 32 * RS_DL + (r & 31)];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0.;
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) sum += red[i];
+    a.dlam[head] = (float)-sum;
+  }
+}
+__global__ __launch_bounds__(1024) void da_dlam(const DaArgs a) { head_dlam(a, blockIdx.x); }
+
+// dK and dV: a wave owns 32 keys, walks the rows that see them.  Its keys stay in registers, and its values: at D = 128, where
+// the accumulators alone are 256 registers, in LDS.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void da_bwd_kv(const DaArgs a) {
-  constexpr int CH = D / 4, DV = 2 * D, NT = 64 * NW, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32;
-  constexpr bool HALF = __is_same(T, _Float16);
+  constexpr bool VLDS = D == 128;
+  constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32, TILE = Stage<T, D, NW>::TILE;
+  constexpr bool HALF = DsScale<T>::ON;
   constexpr float PS = HALF ? 1024.f : 1.f;       // |P_1 - lam P_2| <= max(1, |lam|): keeps fp16's P out of the subnormals
+  typedef Stage<T, D, NW> St;
   typedef typename Vec<T>::v8 v8;
-  __shared__ __align__(16) T qs[32 * DV], gs[32 * DV];
-  __shared__ __align__(16) float st[5][32];
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-  const int tile = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles;
+  __shared__ __align__(1024) T tiles[2][TILE];
+  __shared__ __align__(16) float stats[2][RS_LINES * 32];
+  __shared__ __align__(16) T vlds[VLDS ? NW * 32 * DV : 8];
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nbh = a.B * a.Hkv;
+  const Stage<T, D, NW> plan(wave, lane);
+  // pairs of tiles that are far apart come half the grid apart: causal halves of the work meet on a compute unit
+  const int bh = blockIdx.x % nbh, ord = blockIdx.x / nbh, half = (a.tiles + 1) / 2;
+  const int tile = ord < half ? ord : a.tiles - 1 - (ord - half);
   const Seq s(a, bh);
   const int kb = tile * 32 * NW, key = kb + wave * 32 + (lane & 31), kr = min(key, a.S - 1);
+  // rows that see a key of the block: positions from t0 to the sequence's end
+  const int t0 = kb >= s.kl ? s.ql : a.causal ? max(0, kb - (s.kl - s.ql)) : 0;
+  const int r0 = t0 * a.G / 32 * 32, r1 = s.ql * a.G;
+  const auto stage = [&](int rb, int cur) {
+    const int tb = rb / a.G;
+    const auto qb = (const T*)a.q + s.b * a.q_sb + tb * a.q_st + s.hk * a.G * a.q_sh;
+    const auto gb = (const T*)a.dout + s.b * a.g_sb + tb * a.g_st + s.hk * a.G * a.g_sh;
+#pragma unroll
+    for (int i = 0; i < St::ROLES; ++i) {
+      const int role = i * NW + wave, step = St::step(role);
+      const auto rs = open_range(role < 2 ? qb + (role ? a.q_sc : 0) : gb);
+      const int st = (int)((role < 2 ? a.q_st : a.g_st) * sizeof(T)), sh = (int)((role < 2 ? a.q_sh : a.g_sh) * sizeof(T));
+#pragma unroll
+      for (int j = 0; j < St::PER; ++j) {
+        const int r = rb + plan.row[i] + j * step, t = r / a.G, g = r - t * a.G;
+        dma16(rs, tiles[cur] + St::panel_offset(role) + j * 512, r < r1 ? (t - tb) * st + g * sh + plan.byte[i][j] : BUF_OOB);
+      }
+    }
+    if (wave == 0) dma16(open_range(a.part + ((long)bh * a.tiles32 + rb / 32) * (RS_LINES * 32)), stats[cur], lane * 16);
+  };
+  if (r0 < r1) stage(r0, 0);
   const T* kp = (const T*)a.k + s.b * a.k_sb + s.hk * a.k_sh + (long)kr * a.k_ss;
   const T* vp = (const T*)a.v + s.b * a.v_sb + s.hk * a.v_sh + (long)kr * a.v_ss;
-  v8 kf[2][KQ], vf[KV];
+  v8 kf[2][KQ], vf[VLDS ? 1 : KV];
+  T* vown = vlds + (VLDS ? wave * 32 * DV : 0);
 #pragma unroll
   for (int k = 0; k < KQ; ++k) {
     kf[0][k] = *(const v8*)(kp + 16 * k + 8 * h);
     kf[1][k] = *(const v8*)(kp + a.k_sc + 16 * k + 8 * h);
   }
+  if constexpr (VLDS) {
 #pragma unroll
-  for (int k = 0; k < KV; ++k) vf[k] = *(const v8*)(vp + 16 * k + 8 * h);
+    for (int k = 0; k < KV; ++k) {
+      const int r = lane & 31;
+      *(v8*)(vown + r * DV + ((2 * k + h) ^ turn<DV / 8>(r)) * 8) = *(const v8*)(vp + 16 * k + 8 * h);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < KV; ++k) vf[k] = *(const v8*)(vp + 16 * k + 8 * h);
+  }
   f32x16 dk[2][NQ], dv[NO];
 #pragma unroll
   for (int j = 0; j < NQ; ++j) dk[0][j] = dk[1][j] = 0.f;
 #pragma unroll
   for (int j = 0; j < NO; ++j) dv[j] = 0.f;
   DsScale<T> fit;
-  // rows that see a key of the block: positions from t0 to the sequence's end
-  const int t0 = kb >= s.kl ? s.ql : a.causal ? max(0, kb - (s.kl - s.ql)) : 0;
-  const int r1 = s.ql * a.G;
-  for (int rb = t0 * a.G / 32 * 32; rb < r1; rb += 32) {
-    __syncthreads();
-    const int valid = min(32, r1 - rb);
-    const auto q_row = [&](int r) {
-      const int t = (rb + r) / a.G, head = s.hk * a.G + rb + r - t * a.G;
-      return (const T*)a.q + s.b * a.q_sb + t * a.q_st + head * a.q_sh;
-    };
-    const auto g_row = [&](int r) {
-      const int t = (rb + r) / a.G, head = s.hk * a.G + rb + r - t * a.G;
-      return (const T*)a.dout + s.b * a.g_sb + t * a.g_st + head * a.g_sh;
-    };
-    load_tile<T, CH, NT>(qs, valid, a.q_sc, q_row);
-    load_tile<T, CH, NT>(gs, valid, D, g_row);
-    if (threadIdx.x < 32) {
-      const int r = threadIdx.x;
-      const long n = (long)bh * a.R + rb + r;
-      const bool on = r < valid;
-      st[0][r] = on ? a.stat[n] : INFINITY;
-      st[1][r] = on ? a.stat[a.rows + n] : INFINITY;
-      st[2][r] = on ? a.stat[2 * a.rows + n] : 0.f;
-      st[3][r] = on ? a.stat[3 * a.rows + n] : 0.f;
-      st[4][r] = on ? a.lam[s.hk * a.G + (rb + r) % a.G] : 0.f;
-    }
-    __syncthreads();
+  const uint32_t qcol = col_base<T, D>(tiles[0], lane), gcol = col_base<T, DV>(tiles[0] + 64 * D, lane);
+  int cur = 0;
+  for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
+    tile_ready();
+    if (rb + 32 < r1) stage(rb + 32, cur ^ 1);
+    const T* qs = tiles[cur];
+    const T* gs = qs + 64 * D;
+    const float* st = stats[cur];
     f32x16 sc[2], dp = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       sc[c] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, CH>(qs, c * KQ + k, lane), kf[c][k], sc[c]);
+      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, D>(qs + c * 32 * D, k, lane), kf[c][k], sc[c]);
     }
 #pragma unroll
-    for (int k = 0; k < KV; ++k) dp = Mfma<T>::run(frag_row<T, CH>(gs, k, lane), vf[k], dp);
+    for (int k = 0; k < KV; ++k) {
+      if constexpr (VLDS) dp = Mfma<T>::run(frag_row<T, DV>(gs, k, lane), frag_row<T, DV>(vown, k, lane), dp);
+      else dp = Mfma<T>::run(frag_row<T, DV>(gs, k, lane), vf[k], dp);
+    }
     // a row below the diagonal of the wave's last key, or a key behind the end, needs the mask
     const bool edge = kb + wave * 32 + 32 > s.kl || (a.causal && rb / a.G + s.kl - s.ql < kb + wave * 32 + 31);
     f32x16 pc;
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
-      const f32x4 l1 = *(const f32x4*)&st[0][8 * r4 + 4 * h], l2 = *(const f32x4*)&st[1][8 * r4 + 4 * h],
-                  d1 = *(const f32x4*)&st[2][8 * r4 + 4 * h], d2 = *(const f32x4*)&st[3][8 * r4 + 4 * h],
-                  lm = *(const f32x4*)&st[4][8 * r4 + 4 * h];
+      const int at = 8 * r4 + 4 * h;
+      const f32x4 l1 = *(const f32x4*)(st + 32 * RS_L1 + at), l2 = *(const f32x4*)(st + 32 * RS_L2 + at),
+                  d1 = *(const f32x4*)(st + 32 * RS_D1 + at), d2 = *(const f32x4*)(st + 32 * RS_D2 + at),
+                  lm = *(const f32x4*)(st + 32 * RS_LAM + at);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * r4 + j;
-        const bool seen = !edge || key < s.limit(a, (rb + c_row(r, h)) / a.G);
-        const float p1 = seen ? __builtin_amdgcn_exp2f(fmaf(sc[0][r], a.c, -l1[j])) : 0.f;
-        const float p2 = seen ? lm[j] * __builtin_amdgcn_exp2f(fmaf(sc[1][r], a.c, -l2[j])) : 0.f;
-        pc[r] = (p1 - p2) * PS;
-        sc[0][r] = seen ? p1 * (dp[r] - d1[j]) : 0.f;
-        sc[1][r] = seen ? p2 * (d2[j] - dp[r]) : 0.f;
+        sc[0][r] = __builtin_amdgcn_exp2f(fmaf(sc[0][r], a.c, -l1[j]));
+        sc[1][r] = lm[j] * __builtin_amdgcn_exp2f(fmaf(sc[1][r], a.c, -l2[j]));
+      }
+      if (edge) {
+        const i32x4 lim = *(const i32x4*)(st + 32 * RS_LIM + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool seen = key < lim[j];
+          const int r = 4 * r4 + j;
+          sc[0][r] = seen ? sc[0][r] : 0.f;
+          sc[1][r] = seen ? sc[1][r] : 0.f;
+          dp[r] = seen ? dp[r] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * r4 + j;
+        pc[r] = (sc[0][r] - sc[1][r]) * PS;
+        sc[0][r] *= dp[r] - d1[j];
+        sc[1][r] *= d2[j] - dp[r];
       }
     }
     const float down = fit.fit(sc[0], sc[1]);
@@ -529,18 +787,12 @@ __global__ __launch_bounds__(64 * NW, 1) void da_bwd_kv(const DaArgs a) {
       sc[0] *= fit.f;
       sc[1] *= fit.f;
     }
+    const v8 pf[2] = {pack<T>(pc, 0), pack<T>(pc, 1)};
+    const v8 df[2][2] = {{pack<T>(sc[0], 0), pack<T>(sc[0], 1)}, {pack<T>(sc[1], 0), pack<T>(sc[1], 1)}};
+    const uint32_t at = cur * TILE * sizeof(T);
+    add_cols<T, DV>(gcol + at, pf, dv);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const v8 pf = pack<T>(pc, i);
-#pragma unroll
-      for (int j = 0; j < NO; ++j) dv[j] = Mfma<T>::run(frag_col<T, CH>(gs, 16 * i, 32 * j, lane), pf, dv[j]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const v8 df = pack<T>(sc[c], i);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) dk[c][j] = Mfma<T>::run(frag_col<T, CH>(qs, 16 * i, c * D + 32 * j, lane), df, dk[c][j]);
-      }
-    }
+    for (int c = 0; c < 2; ++c) add_cols<T, D>(qcol + at + c * 32 * D * sizeof(T), df[c], dk[c]);
   }
   if (key >= a.S) return;
   const long out = ((long)(s.b * a.S + key) * a.Hkv + s.hk) * DV;
@@ -567,35 +819,16 @@ __global__ __launch_bounds__(64 * NW, 1) void da_bwd_kv(const DaArgs a) {
     }
 }
 
-// dlam of a head: minus the sum over its rows, in fp64, in a fixed order
-__global__ __launch_bounds__(1024) void da_dlam(const DaArgs a, float* __restrict__ dlam) {
-  __shared__ double red[16];
-  const int head = blockIdx.x, hk = head / a.G, g = head - hk * a.G;
-  double v = 0.;
-  const long total = (long)a.B * a.T;
-  for (long i = threadIdx.x; i < total; i += 1024) {
-    const long b = i / a.T, t = i - b * a.T;
-    v += a.dlrow[(b * a.Hkv + hk) * a.R + t * a.G + g];
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double sum = 0.;
-    for (int i = 0; i < 16; ++i) sum += red[i];
-    dlam[head] = (float)-sum;
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ host side
-// four waves share a key tile where that still gives every compute unit a workgroup; else a wave is one by itself
-bool da_wide(long rows_per_bh, long bh) { return cdiv(rows_per_bh, 128) * bh >= 256; }
+// Two pairs of waves share a key tile where the rows fill them; a few rows over many keys are one pair.
+bool da_wide(long rows) { return rows > 32; }
 
+// Key splits that give every compute unit two workgroups of four waves, or four of two, with at least 128 keys each
 int da_splits(const ctr_diffattn_t* p) {
   const int R = p->T * (p->H / p->Hkv);
-  const long bh = (long)p->B * p->Hkv, blocks = da_wide(R, bh) ? cdiv(R, 128) * bh : cdiv(R, 32) * bh;
-  return (int)std::max<long>(1, std::min<long>(1024 / std::max<long>(1, blocks), cdiv(p->S, 128)));
+  const bool wide = da_wide(R);
+  const long blocks = (long)cdiv(R, wide ? 64 : 32) * p->B * p->Hkv;
+  return (int)std::max<long>(1, std::min<long>((wide ? 512 : 1024) / std::max<long>(1, blocks), p->S / 128));
 }
 
 int da_check(const ctr_diffattn_t* p, bool bwd) {
@@ -609,15 +842,17 @@ int da_check(const ctr_diffattn_t* p, bool bwd) {
   CTR_REQUIRE(p->scale > 0.f && std::isfinite(p->scale), "scale > 0");
   if ((long)p->B * p->T == 0 && !(bwd && (long)p->B * p->S > 0)) return 0;
   CTR_REQUIRE(p->lam, "null lam");
-  const auto ok = [](const void* q, std::initializer_list<long> st) {
+  // the row stride is held to what 32 rows' 32-bit byte offsets can reach
+  const auto ok = [](const void* q, std::initializer_list<long> st, long row, long head) {
     if (!q || (uintptr_t)q % 16) return false;
     for (long s : st)
-      if (s % 8) return false;
-    return true;
+      if (s % 8 || s < 0) return false;
+    return row < (1L << 24) && head < (1L << 24);
   };
-  CTR_REQUIRE((long)p->B * p->T == 0 || ok(p->q, {p->q_sb, p->q_st, p->q_sh, p->q_sc}), "q: 16-byte aligned rows");
-  CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->k, {p->k_sb, p->k_ss, p->k_sh, p->k_sc}), "k: 16-byte aligned rows");
-  CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->v, {p->v_sb, p->v_ss, p->v_sh}), "v: 16-byte aligned rows");
+  const long G = p->H / p->Hkv;
+  CTR_REQUIRE((long)p->B * p->T == 0 || ok(p->q, {p->q_sb, p->q_st, p->q_sh, p->q_sc}, p->q_st, G > 1 ? p->q_sh * std::min(32L, G) / 16 : 0), "q: 16-byte aligned rows");
+  CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->k, {p->k_sb, p->k_ss, p->k_sh, p->k_sc}, p->k_ss, 0), "k: 16-byte aligned rows");
+  CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->v, {p->v_sb, p->v_ss, p->v_sh}, p->v_ss, 0), "v: 16-byte aligned rows");
   CTR_REQUIRE((long)p->B * p->T == 0 || (p->o && (uintptr_t)p->o % 16 == 0 && (uintptr_t)p->o2 % 16 == 0), "output");
   return 0;
 }
@@ -642,30 +877,31 @@ DaArgs da_args(const ctr_diffattn_t* p) {
 template <typename T, int D>
 int da_run_fwd(DaArgs a, hipStream_t s) {
   const long bh = (long)a.B * a.Hkv;
-  const bool wide = da_wide(a.R, bh);
-  a.tiles = cdiv(a.R, wide ? 128 : 32);
+  const bool wide = da_wide(a.R);
+  a.tiles = cdiv(a.R, wide ? 64 : 32);
   const long blocks = a.tiles * bh * a.splits;
-  if (wide) da_fwd<T, D, 4><<<(unsigned)blocks, 256, 0, s>>>(a);
-  else da_fwd<T, D, 1><<<(unsigned)blocks, 64, 0, s>>>(a);
-  if (a.splits > 1) da_join<T, D><<<(unsigned)a.rows, 64, 0, s>>>(a);
+  if (wide) da_fwd<T, D, 2><<<(unsigned)blocks, 256, 0, s>>>(a);
+  else da_fwd<T, D, 1><<<(unsigned)blocks, 128, 0, s>>>(a);
+  if (a.splits > 1) da_join<T, D><<<dim3((unsigned)a.rows, 2 * D / 32), 256, 0, s>>>(a);
   return check_launch("diffattn_fwd");
 }
 
 template <typename T, int D>
-int da_run_bwd(DaArgs a, float* dlam, hipStream_t s) {
+int da_run_bwd(DaArgs a, hipStream_t s) {
   const long bh = (long)a.B * a.Hkv;
-  const bool wq = da_wide(a.R, bh), wk = da_wide(a.S, bh);
+  a.tiles32 = cdiv(a.R, 32);
   if (a.rows > 0) {
-    a.tiles = cdiv(a.R, wq ? 128 : 32);
-    if (wq) da_bwd_q<T, D, 4><<<(unsigned)(a.tiles * bh), 256, 0, s>>>(a);
+    const bool wide = a.R > 64;
+    a.tiles = cdiv(a.R, wide ? 128 : 32);
+    if (wide) da_bwd_q<T, D, 4><<<(unsigned)(a.tiles * bh), 256, 0, s>>>(a);
     else da_bwd_q<T, D, 1><<<(unsigned)(a.tiles * bh), 64, 0, s>>>(a);
   }
   if (bh * a.S > 0) {
-    a.tiles = cdiv(a.S, wk ? 128 : 32);
-    if (wk) da_bwd_kv<T, D, 4><<<(unsigned)(a.tiles * bh), 256, 0, s>>>(a);
-    else da_bwd_kv<T, D, 1><<<(unsigned)(a.tiles * bh), 64, 0, s>>>(a);
+    constexpr int NW = D == 128 ? 4 : 2;
+    a.tiles = cdiv(a.S, 32 * NW);
+    da_bwd_kv<T, D, NW><<<(unsigned)(a.tiles * bh), 64 * NW, 0, s>>>(a);
   }
-  da_dlam<<<a.H, 1024, 0, s>>>(a, dlam);
+  da_dlam<<<a.H, 1024, 0, s>>>(a);
   return check_launch("diffattn_bwd");
 }
 
@@ -703,7 +939,8 @@ extern "C" int ctr_diffattn_fwd(const ctr_diffattn_t* p, void* ws, size_t ws_byt
 }
 
 extern "C" size_t ctr_diffattn_bwd_ws_size(const ctr_diffattn_t* p) {
-  return p && p->B > 0 && p->T > 0 ? (size_t)p->B * p->T * p->H * sizeof(float) : 0;
+  if (!p || p->B <= 0 || p->T <= 0 || p->Hkv <= 0 || p->H < p->Hkv) return 0;
+  return (size_t)p->B * p->Hkv * cdiv((long)p->T * (p->H / p->Hkv), 32) * RS_LINES * 32 * sizeof(float);
 }
 
 extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long g_sb, long g_st, long g_sh, void* dq, void* dk,
@@ -712,7 +949,8 @@ extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long 
   CTR_REQUIRE(dlam, "null dlam");
   const bool q_on = (long)p->B * p->T > 0, k_on = (long)p->B * p->S > 0;
   CTR_REQUIRE(!q_on || (p->o2 && p->stat && dq && dout), "null operand");
-  CTR_REQUIRE(!q_on || ((uintptr_t)dout % 16 == 0 && g_sb % 8 == 0 && g_st % 8 == 0 && g_sh % 8 == 0), "dout: 16-byte aligned rows");
+  CTR_REQUIRE(!q_on || ((uintptr_t)dout % 16 == 0 && g_sb % 8 == 0 && g_st % 8 == 0 && g_sh % 8 == 0 && g_sb >= 0 &&
+                        g_st >= 0 && g_sh >= 0 && g_st < (1L << 24) && g_sh * (p->H / p->Hkv > 1) < (1L << 24)), "dout: 16-byte aligned rows");
   CTR_REQUIRE(!k_on || (dk && dv), "null operand");
   CTR_REQUIRE(((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0, "gradients: 16-byte aligned");
   CTR_REQUIRE(ws_bytes >= ctr_diffattn_bwd_ws_size(p), "workspace too small");
@@ -724,8 +962,9 @@ extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long 
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
-  a.dlrow = (float*)ws;
-#define DA_CALL(T, D) da_run_bwd<T, D>(a, dlam, (hipStream_t)stream)
+  a.part = (float*)ws;
+  a.dlam = dlam;
+#define DA_CALL(T, D) da_run_bwd<T, D>(a, (hipStream_t)stream)
   DA_TYPES(DA_CALL);
 #undef DA_CALL
 }

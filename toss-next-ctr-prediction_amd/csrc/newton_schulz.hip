@@ -607,8 +607,11 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
   }
   CTR_REQUIRE(ws_bytes >= ctr_newton_schulz_ws_size(mats, count), "workspace too small");
   hipStream_t s = (hipStream_t)stream;
-  CTR_REQUIRE(ns_allow_lds(), "LDS size attribute");
 
+  bool any = false;
+  for (int i = 0; i < count; ++i) any |= mats[i].rows > 0 && mats[i].cols > 0;
+  if (!any) return 0;
+  CTR_REQUIRE(ns_allow_lds(), "LDS size attribute");
   NsSmallArgs small = {a, b, c, eps, steps, {}};
   int ns = 0;
   size_t small_lds = 0;

@@ -230,7 +230,7 @@ def diff_attention_fwd(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_l
     a.o = out.data_ptr()
     if save:
         o2 = torch.empty_like(out)
-        stat = torch.empty((4, a.B * a.H * a.T), dtype=torch.float32, device=q.device)
+        stat = torch.empty((2, a.B * a.H * a.T), dtype=torch.float32, device=q.device)
         a.o2, a.stat = o2.data_ptr(), stat.data_ptr()
         saved = (o2, stat)
     if out.numel():
@@ -251,11 +251,10 @@ def diff_attention_bwd(dout, q, k, v, lam, out, saved, causal=False, scale=None,
     for t, what in ((dout, "dout"), (out, "out"), (o2, "saved")):
         if tuple(t.shape) != shape or t.dtype != q.dtype:
             raise ValueError(f"diff_attention_bwd: {what} of shape {shape} {q.dtype}, got {tuple(t.shape)} {t.dtype}")
-    if tuple(stat.shape) != (4, a.B * a.H * a.T) or stat.dtype != torch.float32:
+    if tuple(stat.shape) != (2, a.B * a.H * a.T) or stat.dtype != torch.float32:
         raise ValueError("diff_attention_bwd: saved as diff_attention_fwd gave it")
     _device("diff_attention_bwd", q, dout, out, o2, stat)
     dout, out, o2 = _aligned(dout), out.contiguous(), o2.contiguous()
-    stat = stat.clone()         # the kernels put the rows' sums there: two backward passes may run from one forward
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
     dv = torch.empty(v.shape, dtype=q.dtype, device=q.device)
