@@ -36,7 +36,8 @@ struct DaArgs {
   float* stat;                   // 2 planes of rows: log2 sums of the maps
   void *dq, *dk, *dv;
   float* dlam;
-  float* part;                   // forward, split keys: partial results; backward: row statistics (ROWSTAT)
+  float* part;                   // forward, split keys: partial results; backward: row statistics (RS_*)
+  float* kvpart;                 // backward, split rows: partial dK, dV
   const int *q_lens, *kv_lens;
   long q_sb, q_st, q_sh, q_sc, k_sb, k_ss, k_sh, k_sc, v_sb, v_ss, v_sh, g_sb, g_st, g_sh;
   long rows;                     // B Hkv R
@@ -168,20 +169,25 @@ typedef __attribute__((address_space(3))) void lds_void;
 // 64 lanes x 16 bytes, whose LDS places are consecutive.
 template <typename T, int D, int NW>
 struct Stage {
-  static constexpr int PER = D / 16, TILE = 32 * 4 * D, ROLES = 4 / NW;      // TILE: elements of the three panels
+  static constexpr int ROLES = NW >= 4 ? 1 : 4 / NW, SHARE = NW > 4 ? NW / 4 : 1;      // roles of a wave, waves of a role
+  static constexpr int PER = D / 16 / SHARE, TILE = 32 * 4 * D;      // a wave's loads for a role; elements of the three panels
   int row[ROLES], byte[ROLES][PER];      // the lane's row for load 0 of its roles, and its byte in the row for each load
-  static __device__ __forceinline__ int panel_offset(int role) { return role < 2 ? role * 32 * D : 64 * D + (role - 2) * 32 * D; }
+  static __device__ __forceinline__ int role(int i, int wave) { return SHARE > 1 ? wave & 3 : i * NW + wave; }
+  // where a wave's loads for a role begin in LDS (elements)
+  static __device__ __forceinline__ int place(int role, int wave) {
+    return (role < 2 ? role * 32 * D : 64 * D + (role - 2) * 32 * D) + (SHARE > 1 ? (wave >> 2) * PER * 512 : 0);
+  }
   static __device__ __forceinline__ int step(int role) { return role < 2 ? 512 / D : 256 / D; }      // rows from load to load
   __device__ __forceinline__ Stage(int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < ROLES; ++i) {
-      const int role = i * NW + wave;
-      const bool map = role < 2;
-      row[i] = map ? lane / (D / 8) : lane / (D / 4) + (role - 2) * 16;
+      const int ro = role(i, wave);
+      const bool map = ro < 2;
+      row[i] = (map ? lane / (D / 8) : lane / (D / 4) + (ro - 2) * 16) + (SHARE > 1 ? (wave >> 2) * PER * step(ro) : 0);
       const int c = map ? lane % (D / 8) : lane % (D / 4);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const int r = row[i] + j * step(role);
+        const int r = row[i] + j * step(ro);
         byte[i][j] = (c ^ (map ? turn<D / 8>(r) : turn<D / 4>(r))) * 16;
       }
     }
@@ -208,11 +214,11 @@ __device__ __forceinline__ void stage_keys(const DaArgs& a, const Stage<T, D, NW
   typedef Stage<T, D, NW> St;
 #pragma unroll
   for (int i = 0; i < St::ROLES; ++i) {
-    const int role = i * NW + wave;
+    const int role = St::role(i, wave);
     const T* base = role < 2 ? kp + (long)kb * a.k_ss + (role ? a.k_sc : 0) : vp + (long)kb * a.v_ss;
     const int stride = (int)((role < 2 ? a.k_ss : a.v_ss) * sizeof(T)), step = St::step(role);
     const auto rs = open_range(base);
-    T* dst = buf + St::panel_offset(role);
+    T* dst = buf + St::place(role, wave);
     int row = p.row[i], off = row * stride;
     if (valid >= 32) {
 #pragma unroll
@@ -223,6 +229,14 @@ __device__ __forceinline__ void stage_keys(const DaArgs& a, const Stage<T, D, NW
         dma16(rs, dst + j * 512, row < valid ? off + p.byte[i][j] : BUF_OOB);
     }
   }
+}
+
+// every wave's LDS writes before it are seen after it; loads in flight stay in flight
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 struct Seq {
@@ -486,11 +500,14 @@ struct DsScale {
 template <typename T, int W, int N>
 __device__ __forceinline__ void add_cols(uint32_t base, const typename Vec<T>::v8 (&x)[2], f32x16 (&acc)[N]) {
   static_assert(N == W / 32, "panel");
-  if constexpr (N == 1) {
-    typename Vec<T>::v8 f[2];
-    frag_col1<T, W>(base, f);
-    acc[0] = Mfma<T>::run(f[0], x[0], acc[0]);
-    acc[0] = Mfma<T>::run(f[1], x[1], acc[0]);
+  if constexpr (N == 1 || N == 8) {       // eight tiles leave no registers for two groups
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      typename Vec<T>::v8 f[2];
+      frag_col1<T, W>(base ^ (j << 6), f);
+      acc[j] = Mfma<T>::run(f[0], x[0], acc[j]);
+      acc[j] = Mfma<T>::run(f[1], x[1], acc[j]);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
@@ -656,167 +673,198 @@ __device__ __forceinline__ void head_dlam(const DaArgs& a, int head) {
 }
 __global__ __launch_bounds__(1024) void da_dlam(const DaArgs a) { head_dlam(a, blockIdx.x); }
 
-// dK and dV: a wave owns 32 keys, walks the rows that see them.  Its keys stay in registers, and its values: at D = 128, where
-// the accumulators alone are 256 registers, in LDS.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void da_bwd_kv(const DaArgs a) {
-  constexpr bool VLDS = D == 128;
-  constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32, TILE = Stage<T, D, NW>::TILE;
+// dK and dV of 32 keys a pair of waves, NP pairs a workgroup, walking the rows that see them.  The pair divides the work, with
+// the same number of matrix instructions each: the first wave forms the maps and dV = (P_1 - lam P_2)^T dO, the second
+// dP, dS and dK_c = dS_c^T Q_c; the probabilities pass from one to the other through LDS in fp32, once a tile.  Each so
+// holds half of the accumulators and two waves fit a SIMD: one's exponentials run under the other's products.
+template <typename T, int D, int NP>
+__global__ __launch_bounds__(128 * NP, 2) void da_bwd_kv(const DaArgs a) {
+  constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32, NW = 2 * NP, TILE = Stage<T, D, NW>::TILE;
   constexpr bool HALF = DsScale<T>::ON;
   constexpr float PS = HALF ? 1024.f : 1.f;       // |P_1 - lam P_2| <= max(1, |lam|): keeps fp16's P out of the subnormals
   typedef Stage<T, D, NW> St;
   typedef typename Vec<T>::v8 v8;
   __shared__ __align__(1024) T tiles[2][TILE];
   __shared__ __align__(16) float stats[2][RS_LINES * 32];
-  __shared__ __align__(16) T vlds[VLDS ? NW * 32 * DV : 8];
+  __shared__ __align__(16) f32x4 probs[NP][2][4][64];
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nbh = a.B * a.Hkv;
-  const Stage<T, D, NW> plan(wave, lane);
-  // pairs of tiles that are far apart come half the grid apart: causal halves of the work meet on a compute unit
-  const int bh = blockIdx.x % nbh, ord = blockIdx.x / nbh, half = (a.tiles + 1) / 2;
-  const int tile = ord < half ? ord : a.tiles - 1 - (ord - half);
+  const int pair = wave % NP;
+  const St plan(wave, lane);
+  // the causally longest come first
+  const int bh = blockIdx.x % nbh, tile = blockIdx.x / nbh / a.splits, sp = blockIdx.x / nbh % a.splits;
   const Seq s(a, bh);
-  const int kb = tile * 32 * NW, key = kb + wave * 32 + (lane & 31), kr = min(key, a.S - 1);
+  const int kb = tile * 32 * NP, kw = kb + pair * 32, key = kw + (lane & 31), kr = min(key, a.S - 1);
   // rows that see a key of the block: positions from t0 to the sequence's end
   const int t0 = kb >= s.kl ? s.ql : a.causal ? max(0, kb - (s.kl - s.ql)) : 0;
-  const int r0 = t0 * a.G / 32 * 32, r1 = s.ql * a.G;
+  int r0 = t0 * a.G / 32 * 32, r1 = s.ql * a.G;
+  if (a.splits > 1) {              // this split's share of them
+    const int per = (max(0, r1 - r0) / 32 + a.splits) / a.splits * 32;
+    r0 += sp * per;
+    r1 = min(r1, r0 + per);
+  }
   const auto stage = [&](int rb, int cur) {
     const int tb = rb / a.G;
     const auto qb = (const T*)a.q + s.b * a.q_sb + tb * a.q_st + s.hk * a.G * a.q_sh;
     const auto gb = (const T*)a.dout + s.b * a.g_sb + tb * a.g_st + s.hk * a.G * a.g_sh;
 #pragma unroll
     for (int i = 0; i < St::ROLES; ++i) {
-      const int role = i * NW + wave, step = St::step(role);
+      const int role = St::role(i, wave), step = St::step(role);
       const auto rs = open_range(role < 2 ? qb + (role ? a.q_sc : 0) : gb);
       const int st = (int)((role < 2 ? a.q_st : a.g_st) * sizeof(T)), sh = (int)((role < 2 ? a.q_sh : a.g_sh) * sizeof(T));
 #pragma unroll
       for (int j = 0; j < St::PER; ++j) {
         const int r = rb + plan.row[i] + j * step, t = r / a.G, g = r - t * a.G;
-        dma16(rs, tiles[cur] + St::panel_offset(role) + j * 512, r < r1 ? (t - tb) * st + g * sh + plan.byte[i][j] : BUF_OOB);
+        dma16(rs, tiles[cur] + St::place(role, wave) + j * 512, r < r1 ? (t - tb) * st + g * sh + plan.byte[i][j] : BUF_OOB);
       }
     }
     if (wave == 0) dma16(open_range(a.part + ((long)bh * a.tiles32 + rb / 32) * (RS_LINES * 32)), stats[cur], lane * 16);
   };
   if (r0 < r1) stage(r0, 0);
-  const T* kp = (const T*)a.k + s.b * a.k_sb + s.hk * a.k_sh + (long)kr * a.k_ss;
-  const T* vp = (const T*)a.v + s.b * a.v_sb + s.hk * a.v_sh + (long)kr * a.v_ss;
-  v8 kf[2][KQ], vf[VLDS ? 1 : KV];
-  T* vown = vlds + (VLDS ? wave * 32 * DV : 0);
+  const long out = ((long)s.b * a.S + key) * a.Hkv + s.hk;
+  // four elements of the key's dK (from 0) or dV (from DV), or of their part
+  const auto put = [&](T* to, int from, int c, const f32x4& x) {
+    if (a.splits > 1) *(f32x4*)(a.kvpart + (((long)sp * a.B * a.S * a.Hkv + out) * 2 * DV + from + c)) = x;
+    else *(typename Vec<T>::v4*)(to + out * DV + c) = __builtin_convertvector(x, typename Vec<T>::v4);
+  };
+  if (wave < NP) {
+    const T* kp = (const T*)a.k + s.b * a.k_sb + s.hk * a.k_sh + (long)kr * a.k_ss;
+    v8 kf[2][KQ];
 #pragma unroll
-  for (int k = 0; k < KQ; ++k) {
-    kf[0][k] = *(const v8*)(kp + 16 * k + 8 * h);
-    kf[1][k] = *(const v8*)(kp + a.k_sc + 16 * k + 8 * h);
-  }
-  if constexpr (VLDS) {
-#pragma unroll
-    for (int k = 0; k < KV; ++k) {
-      const int r = lane & 31;
-      *(v8*)(vown + r * DV + ((2 * k + h) ^ turn<DV / 8>(r)) * 8) = *(const v8*)(vp + 16 * k + 8 * h);
+    for (int k = 0; k < KQ; ++k) {
+      kf[0][k] = *(const v8*)(kp + 16 * k + 8 * h);
+      kf[1][k] = *(const v8*)(kp + a.k_sc + 16 * k + 8 * h);
     }
-  } else {
+    f32x16 dv[NO];
 #pragma unroll
-    for (int k = 0; k < KV; ++k) vf[k] = *(const v8*)(vp + 16 * k + 8 * h);
-  }
-  f32x16 dk[2][NQ], dv[NO];
+    for (int j = 0; j < NO; ++j) dv[j] = 0.f;
+    const uint32_t gcol = col_base<T, DV>(tiles[0] + 64 * D, lane);
+    int cur = 0;
+    for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
+      tile_ready();
+      if (rb + 32 < r1) stage(rb + 32, cur ^ 1);
+      const T* qs = tiles[cur];
+      const float* st = stats[cur];
+      // a row below the diagonal of the pair's last key, or a key behind the end, needs the mask
+      const bool edge = kw + 32 > s.kl || (a.causal && rb / a.G + s.kl - s.ql < kw + 31);
+      f32x16 pc;
 #pragma unroll
-  for (int j = 0; j < NQ; ++j) dk[0][j] = dk[1][j] = 0.f;
+      for (int c = 0; c < 2; ++c) {
+        f32x16 sc = 0.f;
 #pragma unroll
-  for (int j = 0; j < NO; ++j) dv[j] = 0.f;
-  DsScale<T> fit;
-  const uint32_t qcol = col_base<T, D>(tiles[0], lane), gcol = col_base<T, DV>(tiles[0] + 64 * D, lane);
-  int cur = 0;
-  for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
-    tile_ready();
-    if (rb + 32 < r1) stage(rb + 32, cur ^ 1);
-    const T* qs = tiles[cur];
-    const T* gs = qs + 64 * D;
-    const float* st = stats[cur];
-    f32x16 sc[2], dp = 0.f;
+        for (int k = 0; k < KQ; ++k) sc = Mfma<T>::run(frag_row<T, D>(qs + c * 32 * D, k, lane), kf[c][k], sc);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      sc[c] = 0.f;
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int at = 8 * r4 + 4 * h;
+          const f32x4 ls = *(const f32x4*)(st + 32 * (c ? RS_L2 : RS_L1) + at);
+          f32x4 p;
 #pragma unroll
-      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, D>(qs + c * 32 * D, k, lane), kf[c][k], sc[c]);
-    }
+          for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(sc[4 * r4 + j], a.c, -ls[j]));
+          if (c) p *= *(const f32x4*)(st + 32 * RS_LAM + at);
+          if (edge) {
+            const i32x4 lim = *(const i32x4*)(st + 32 * RS_LIM + at);
 #pragma unroll
-    for (int k = 0; k < KV; ++k) {
-      if constexpr (VLDS) dp = Mfma<T>::run(frag_row<T, DV>(gs, k, lane), frag_row<T, DV>(vown, k, lane), dp);
-      else dp = Mfma<T>::run(frag_row<T, DV>(gs, k, lane), vf[k], dp);
-    }
-    // a row below the diagonal of the wave's last key, or a key behind the end, needs the mask
-    const bool edge = kb + wave * 32 + 32 > s.kl || (a.causal && rb / a.G + s.kl - s.ql < kb + wave * 32 + 31);
-    f32x16 pc;
+            for (int j = 0; j < 4; ++j) p[j] = key < lim[j] ? p[j] : 0.f;
+          }
+          probs[pair][c][r4][lane] = p;
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int at = 8 * r4 + 4 * h;
-      const f32x4 l1 = *(const f32x4*)(st + 32 * RS_L1 + at), l2 = *(const f32x4*)(st + 32 * RS_L2 + at),
-                  d1 = *(const f32x4*)(st + 32 * RS_D1 + at), d2 = *(const f32x4*)(st + 32 * RS_D2 + at),
-                  lm = *(const f32x4*)(st + 32 * RS_LAM + at);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 4 * r4 + j;
-        sc[0][r] = __builtin_amdgcn_exp2f(fmaf(sc[0][r], a.c, -l1[j]));
-        sc[1][r] = lm[j] * __builtin_amdgcn_exp2f(fmaf(sc[1][r], a.c, -l2[j]));
-      }
-      if (edge) {
-        const i32x4 lim = *(const i32x4*)(st + 32 * RS_LIM + at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool seen = key < lim[j];
-          const int r = 4 * r4 + j;
-          sc[0][r] = seen ? sc[0][r] : 0.f;
-          sc[1][r] = seen ? sc[1][r] : 0.f;
-          dp[r] = seen ? dp[r] : 0.f;
+          for (int j = 0; j < 4; ++j) pc[4 * r4 + j] = c ? pc[4 * r4 + j] - p[j] : p[j];
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 4 * r4 + j;
-        pc[r] = (sc[0][r] - sc[1][r]) * PS;
-        sc[0][r] *= dp[r] - d1[j];
-        sc[1][r] *= d2[j] - dp[r];
-      }
+      if constexpr (HALF) pc *= PS;
+      const v8 pf[2] = {pack<T>(pc, 0), pack<T>(pc, 1)};
+      lds_barrier();
+      add_cols<T, DV>(gcol + cur * TILE * sizeof(T), pf, dv);
     }
-    const float down = fit.fit(sc[0], sc[1]);
-    if (down != 1.f) {
+    if (key >= a.S) return;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) dk[c][j] *= down;
-    }
-    if constexpr (HALF) {
-      sc[0] *= fit.f;
-      sc[1] *= fit.f;
-    }
-    const v8 pf[2] = {pack<T>(pc, 0), pack<T>(pc, 1)};
-    const v8 df[2][2] = {{pack<T>(sc[0], 0), pack<T>(sc[0], 1)}, {pack<T>(sc[1], 0), pack<T>(sc[1], 1)}};
-    const uint32_t at = cur * TILE * sizeof(T);
-    add_cols<T, DV>(gcol + at, pf, dv);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) add_cols<T, D>(qcol + at + c * 32 * D * sizeof(T), df[c], dk[c]);
-  }
-  if (key >= a.S) return;
-  const long out = ((long)(s.b * a.S + key) * a.Hkv + s.hk) * DV;
-  const float f = a.scale / fit.f;
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int j = 0; j < NQ; ++j)
+    for (int j = 0; j < NO; ++j)
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        typename Vec<T>::v4 x;
+        f32x4 x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = (T)(dk[c][j][4 * r4 + r] * f);
-        *(typename Vec<T>::v4*)((T*)a.dk + out + c * D + 32 * j + 8 * r4 + 4 * h) = x;
+        for (int r = 0; r < 4; ++r) x[r] = dv[j][4 * r4 + r] * (1.f / PS);
+        put((T*)a.dv, DV, 32 * j + 8 * r4 + 4 * h, x);
+      }
+  } else {
+    const T* vp = (const T*)a.v + s.b * a.v_sb + s.hk * a.v_sh + (long)kr * a.v_ss;
+    v8 vf[KV];
+#pragma unroll
+    for (int k = 0; k < KV; ++k) vf[k] = *(const v8*)(vp + 16 * k + 8 * h);
+    f32x16 dk[2][NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) dk[0][j] = dk[1][j] = 0.f;
+    DsScale<T> fit;
+    const uint32_t qcol = col_base<T, D>(tiles[0], lane);
+    int cur = 0;
+    for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
+      tile_ready();
+      if (rb + 32 < r1) stage(rb + 32, cur ^ 1);
+      const T* gs = tiles[cur] + 64 * D;
+      const float* st = stats[cur];
+      f32x16 dp = 0.f;
+#pragma unroll
+      for (int k = 0; k < KV; ++k) dp = Mfma<T>::run(frag_row<T, DV>(gs, k, lane), vf[k], dp);
+      // dP of a masked place may be anything (a value behind the end): its dS is 0
+      const bool edge = kw + 32 > s.kl;
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = key < s.kl ? dp[r] : 0.f;
+      }
+      lds_barrier();
+      f32x16 ds[2];
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int at = 8 * r4 + 4 * h;
+        const f32x4 d1 = *(const f32x4*)(st + 32 * RS_D1 + at), d2 = *(const f32x4*)(st + 32 * RS_D2 + at);
+        const f32x4 p1 = probs[pair][0][r4][lane], p2 = probs[pair][1][r4][lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * r4 + j;
+          ds[0][r] = p1[j] * (dp[r] - d1[j]);
+          ds[1][r] = p2[j] * (d2[j] - dp[r]);
+        }
+      }
+      const float down = fit.fit(ds[0], ds[1]);
+      if (down != 1.f) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) dk[c][j] *= down;
       }
 #pragma unroll
-  for (int j = 0; j < NO; ++j)
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      typename Vec<T>::v4 x;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = (T)(dv[j][4 * r4 + r] * (1.f / PS));
-      *(typename Vec<T>::v4*)((T*)a.dv + out + 32 * j + 8 * r4 + 4 * h) = x;
+      for (int c = 0; c < 2; ++c) {
+        if constexpr (HALF) ds[c] *= fit.f;
+        const v8 df[2] = {pack<T>(ds[c], 0), pack<T>(ds[c], 1)};
+        add_cols<T, D>(qcol + (cur * TILE + c * 32 * D) * sizeof(T), df, dk[c]);
+      }
     }
+    if (key >= a.S) return;
+    const float f = a.scale / fit.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          f32x4 x;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = dk[c][j][4 * r4 + r] * f;
+          put((T*)a.dk, 0, c * D + 32 * j + 8 * r4 + 4 * h, x);
+        }
+  }
+}
+
+// sums the row splits' dK and dV in order: a thread takes four elements of a key's 2 D + 2 D
+template <typename T, int D>
+__global__ __launch_bounds__(256) void da_kv_join(const DaArgs a) {
+  constexpr int DV = 2 * D;
+  const long n = (long)a.B * a.S * a.Hkv * (2 * DV), i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 v = *(const f32x4*)(a.kvpart + i);
+  for (int s = 1; s < a.splits; ++s) v += *(const f32x4*)(a.kvpart + s * n + i);
+  const long key = i / (2 * DV);
+  const int c = (int)(i - key * (2 * DV));
+  *(typename Vec<T>::v4*)((T*)(c < DV ? a.dk : a.dv) + key * DV + (c < DV ? c : c - DV)) = __builtin_convertvector(v, typename Vec<T>::v4);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -829,6 +877,18 @@ int da_splits(const ctr_diffattn_t* p) {
   const bool wide = da_wide(R);
   const long blocks = (long)cdiv(R, wide ? 64 : 32) * p->B * p->Hkv;
   return (int)std::max<long>(1, std::min<long>((wide ? 512 : 1024) / std::max<long>(1, blocks), p->S / 128));
+}
+
+constexpr int da_pairs(int D) { return D == 128 ? 4 : 2; }
+
+// Row splits of the dK / dV kernel: eight workgroups a compute unit in all, so that the causal differences of their lengths
+// even out, with at least eight row tiles each; a split costs its fp32 part of dK and dV, written and read once.
+int da_kv_splits(const ctr_diffattn_t* p) {
+  const long blocks = (long)cdiv(p->S, 32 * da_pairs(p->D)) * p->B * p->Hkv, tiles = cdiv((long)p->T * (p->H / p->Hkv), 32);
+  return (int)std::max<long>(1, std::min<long>({8, 2048 / std::max<long>(1, blocks), tiles / 8}));
+}
+size_t da_rowstat_bytes(const ctr_diffattn_t* p) {
+  return (size_t)p->B * p->Hkv * cdiv((long)p->T * (p->H / p->Hkv), 32) * RS_LINES * 32 * sizeof(float);
 }
 
 int da_check(const ctr_diffattn_t* p, bool bwd) {
@@ -887,7 +947,7 @@ int da_run_fwd(DaArgs a, hipStream_t s) {
 }
 
 template <typename T, int D>
-int da_run_bwd(DaArgs a, hipStream_t s) {
+int da_run_bwd(DaArgs a, int kv_splits, hipStream_t s) {
   const long bh = (long)a.B * a.Hkv;
   a.tiles32 = cdiv(a.R, 32);
   if (a.rows > 0) {
@@ -897,9 +957,11 @@ int da_run_bwd(DaArgs a, hipStream_t s) {
     else da_bwd_q<T, D, 1><<<(unsigned)(a.tiles * bh), 64, 0, s>>>(a);
   }
   if (bh * a.S > 0) {
-    constexpr int NW = D == 128 ? 4 : 2;
-    a.tiles = cdiv(a.S, 32 * NW);
-    da_bwd_kv<T, D, NW><<<(unsigned)(a.tiles * bh), 64 * NW, 0, s>>>(a);
+    constexpr int NP = da_pairs(D);
+    a.tiles = cdiv(a.S, 32 * NP);
+    a.splits = kv_splits;
+    da_bwd_kv<T, D, NP><<<(unsigned)(a.tiles * bh * a.splits), 128 * NP, 0, s>>>(a);
+    if (a.splits > 1) da_kv_join<T, D><<<(unsigned)cdiv(bh * a.S * 4 * D, 1024), 256, 0, s>>>(a);
   }
   da_dlam<<<a.H, 1024, 0, s>>>(a);
   return check_launch("diffattn_bwd");
@@ -940,7 +1002,8 @@ extern "C" int ctr_diffattn_fwd(const ctr_diffattn_t* p, void* ws, size_t ws_byt
 
 extern "C" size_t ctr_diffattn_bwd_ws_size(const ctr_diffattn_t* p) {
   if (!p || p->B <= 0 || p->T <= 0 || p->Hkv <= 0 || p->H < p->Hkv) return 0;
-  return (size_t)p->B * p->Hkv * cdiv((long)p->T * (p->H / p->Hkv), 32) * RS_LINES * 32 * sizeof(float);
+  const int splits = da_kv_splits(p);
+  return da_rowstat_bytes(p) + (splits > 1 ? (size_t)splits * p->B * p->S * p->Hkv * 4 * p->D * sizeof(float) : 0);
 }
 
 extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long g_sb, long g_st, long g_sh, void* dq, void* dk,
@@ -963,8 +1026,9 @@ extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long 
   a.dk = dk;
   a.dv = dv;
   a.part = (float*)ws;
+  a.kvpart = (float*)((char*)ws + da_rowstat_bytes(p));
   a.dlam = dlam;
-#define DA_CALL(T, D) da_run_bwd<T, D>(a, (hipStream_t)stream)
+#define DA_CALL(T, D) da_run_bwd<T, D>(a, da_kv_splits(p), (hipStream_t)stream)
   DA_TYPES(DA_CALL);
 #undef DA_CALL
 }
