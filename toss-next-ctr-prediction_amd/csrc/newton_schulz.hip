@@ -25,7 +25,7 @@ constexpr int NS_TILE = 128, NS_BK = 32;
 constexpr int LDK = NS_BK + 8, LDN = NS_TILE + 32;   // LDS row strides (elements): k-contiguous tiles, n-contiguous tiles
 constexpr int PLANE_K = NS_TILE * LDK, PLANE_N = NS_BK * LDN;
 static_assert(PLANE_K == PLANE_N, "one LDS plane size");
-constexpr int NS_SUMSQ_BLOCKS = 64;
+constexpr int NS_SUMSQ_BLOCKS = 256;
 constexpr int NS_SMALL_LDS = 160 * 1024 - 256;   // of a workgroup, next to its few static bytes
 
 struct NsMat {
@@ -109,16 +109,30 @@ __device__ __forceinline__ f16x8 frag_t(const _Float16* p, int ld, int k, int co
 }
 
 // ------------------------------------------------------------------------------------------------ large matrices
+template <typename T>
+__device__ __forceinline__ double ns_rows_sumsq(const NsMat& q) {
+  // 8-element pieces of the rows, dealt over all threads; a thread's own sum of 64 squares at a time in fp32 would overflow
+  // where the matrix does not, so fp64 from the start
+  double s = 0.;
+  const int per = (q.cols + 7) / 8;
+  const long total = (long)q.rows * per, step = (long)NS_SUMSQ_BLOCKS * 256;
+  const int dr = (int)(step / per), dc = (int)(step % per);
+  long i = (long)blockIdx.x * 256 + threadIdx.x;
+  int r = (int)(i / per), c = (int)(i % per);
+  for (; i < total; i += step) {
+    const f32x8 v = ld8f((const T*)q.src + (long)r * q.ld_src + c * 8, q.cols - c * 8);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s = fma((double)v[k], (double)v[k], s);
+    r += dr;
+    c += dc;
+    if (c >= per) c -= per, ++r;
+  }
+  return s;
+}
 __global__ __launch_bounds__(256) void ns_sumsq(const NsArgs p) {
   const NsMat& q = p.mat[blockIdx.y];
   __shared__ double red[4];
-  double s = 0.;
-  const long total = (long)q.rows * q.cols;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    const int r = (int)(i / q.cols), c = (int)(i - (long)r * q.cols);
-    const double v = ns_load(q, r, c);
-    s = fma(v, v, s);
-  }
+  double s = q.type == TY_F32 ? ns_rows_sumsq<float>(q) : q.type == TY_BF16 ? ns_rows_sumsq<__bf16>(q) : ns_rows_sumsq<_Float16>(q);
   s = block_sum64(s, red);
   if (threadIdx.x == 0) ((double*)(p.ws + q.off_s))[blockIdx.x] = s;
 }
@@ -247,31 +261,49 @@ __global__ __launch_bounds__(256, 2) void ns_gram(const NsArgs p, int buf) {
             b * 32 + (lane & 31)] = acc[a][b][r];
 }
 
-// the partials of a 32 x 32 block of the lower tiles summed in order, both triangles' planes written
+// the partials of a 32 x 32 block of the lower tiles summed in order (four elements a thread, eight loads in flight), both
+// triangles' planes written
 __global__ __launch_bounds__(256) void ns_gram_join(const NsArgs p) {
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
   __shared__ float tile[32][33];
   int ti, tj;
   tri(blockIdx.x - p.pre[i], ti, tj);
-  const float* in = (const float*)(p.ws + q.off_p);
   _Float16* A = (_Float16*)(p.ws + q.off_a);
   const long plane = (long)q.mp * q.mp;
-  const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
-  for (int j = ly; j < 32; j += 8) {
-    const long o = (long)(ti * 32 + j) * q.mp + tj * 32 + lx;
-    float v = 0.f;
-    for (int s = 0; s < q.splits; ++s) v += in[s * plane + o];
-    v *= SA / (SX * SX);
-    tile[j][lx] = v;
-    split16(v, A[o], A[plane + o]);
+  const int r = threadIdx.x >> 3, c4 = (threadIdx.x & 7) * 4;
+  const float* in = (const float*)(p.ws + q.off_p) + (long)(ti * 32 + r) * q.mp + tj * 32 + c4;
+  f32x4 v = 0.f;
+  int s = 0;
+  for (; s + 8 <= q.splits; s += 8) {
+    f32x4 u[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = *(const f32x4*)(in + (s + k) * plane);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += u[k];
   }
+  for (; s < q.splits; ++s) v += *(const f32x4*)(in + s * plane);
+  v *= SA / (SX * SX);
+  const auto put = [&](int row, int col, const f32x4& x) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      _Float16 a, b;
+      split16(x[k], a, b);
+      hi[k] = a;
+      lo[k] = b;
+    }
+    *(f16x4*)(A + (long)row * q.mp + col) = hi;
+    *(f16x4*)(A + plane + (long)row * q.mp + col) = lo;
+  };
+  put(ti * 32 + r, tj * 32 + c4, v);
   if (ti == tj) return;      // the whole block: it is symmetric by itself
+#pragma unroll
+  for (int k = 0; k < 4; ++k) tile[c4 + k][r] = v[k];
   __syncthreads();
-  for (int j = ly; j < 32; j += 8) {
-    const long o = (long)(tj * 32 + j) * q.mp + ti * 32 + lx;
-    split16(tile[lx][j], A[o], A[plane + o]);
-  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = tile[r][c4 + k];
+  put(tj * 32 + r, ti * 32 + c4, v);
 }
 
 // W = a I + b A + c A A, lower tiles, both triangles written
@@ -359,144 +391,160 @@ struct NsSmallArgs {
   NsMat mat[NS_MAXMAT];
 };
 
-__host__ __device__ inline int ns_small_splits(int mt) { return mt == 1 ? 8 : mt == 2 ? 2 : 1; }
+constexpr int ns_small_splits(int mt) { return mt == 1 ? 8 : mt == 2 ? 2 : 1; }      // of the Gram matrix's columns
 inline size_t ns_small_lds(int mp, int np) {
   const int mt = mp / 32, sp = ns_small_splits(mt);
-  return (size_t)4 * mp * (np + 8) + (size_t)4 * mp * (mp + 8) + (size_t)(sp - 1) * mt * mt * 4096;
+  return (size_t)4 * mp * (np + 8) + (size_t)4 * mp * (mp + 8) + (sp > 1 ? (size_t)sp * mt * mt * 4096 : 0);
 }
 inline bool ns_is_small(int mp, int np) {
   return mp / 32 <= 4 && (mp / 32) * (np / 32) <= 32 && ns_small_lds(mp, np) <= NS_SMALL_LDS;
 }
 
-__global__ __launch_bounds__(512) void ns_small(const NsSmallArgs p) {
-  extern __shared__ __align__(16) _Float16 lds[];
-  __shared__ double red[8];
-  const NsMat& q = p.mat[blockIdx.x];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5;
-  const int mp = q.mp, np = q.np, ldx = np + 8, lda = mp + 8, mt = mp / 32, nt = np / 32;
-  _Float16 *Xh = lds, *Xl = Xh + mp * ldx, *Ah = Xl + mp * ldx, *Al = Ah + mp * lda;
-  float* part = (float*)(Al + mp * lda);
-  const bool tall = q.rows > q.cols;
-  const int total = q.rows * q.cols;
-  double s = 0.;
-  for (int i = t; i < total; i += 512) {
-    const double v = ns_load(q, i / q.cols, i % q.cols);
-    s = fma(v, v, s);
+// a 32 x 32 tile of a product over [k0, k1): rows of A, and rows (NT) or columns (NN) of B; every operand two planes
+template <bool NN>
+__device__ __forceinline__ f32x16 small_tile(const _Float16* Ah, const _Float16* Al, int lda, int r0, const _Float16* Bh,
+                                             const _Float16* Bl, int ldb, int c0, int k0, int k1, int lane) {
+  f32x16 acc = 0.f;
+#pragma unroll 2
+  for (int k = k0; k < k1; k += 16) {
+    const f16x8 ah = NN ? frag_kp(Ah, lda, r0, k, lane) : frag_k(Ah, lda, r0, k, lane),
+                al = NN ? frag_kp(Al, lda, r0, k, lane) : frag_k(Al, lda, r0, k, lane);
+    const f16x8 bh = NN ? frag_t(Bh, ldb, k, c0, lane) : frag_k(Bh, ldb, c0, k, lane),
+                bl = NN ? frag_t(Bl, ldb, k, c0, lane) : frag_k(Bl, ldb, c0, k, lane);
+    acc = MFMA16(al, bh, acc);
+    acc = MFMA16(ah, bl, acc);
+    acc = MFMA16(ah, bh, acc);
   }
+  return acc;
+}
+
+template <typename T, int MT>
+__device__ __forceinline__ void ns_small_run(const NsSmallArgs& p, const NsMat& q, _Float16* lds, double* red) {
+  constexpr int MP = 32 * MT, LDA = MP + 8, SPLITS = ns_small_splits(MT), UNITS = MT * MT * SPLITS, NA = (MT * MT + 7) / 8;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int np = q.np, ldx = np + 8, nt = np / 32;
+  _Float16 *Xh = lds, *Xl = Xh + MP * ldx, *Ah = Xl + MP * ldx, *Al = Ah + MP * LDA;
+  float* part = (float*)(Al + MP * LDA);
+  const bool tall = q.rows > q.cols;
+  const T* src = (const T*)q.src;
+  // the whole matrix in registers (at most 64 elements a thread), all loads in flight at once; e / cols is the upper half of
+  // e ceil(2^32 / cols), exact for e cols < 2^32
+  const int total = q.rows * q.cols;
+  const uint32_t magic = q.cols == 1 ? 0 : (uint32_t)((0x100000000ull + q.cols - 1) / q.cols);
+  const auto row_of = [&](int e) { return q.cols == 1 ? e : (int)__umulhi((uint32_t)e, magic); };
+  float g[64];
+#pragma unroll
+  for (int k = 0; k < 64; ++k) {
+    const int e = t + 512 * k, r = row_of(e);
+    g[k] = e < total ? (float)src[(long)r * q.ld_src + (e - r * q.cols)] : 0.f;
+  }
+  for (int e = t * 8; e < 2 * MP * ldx; e += 4096) *(f16x8*)(Xh + e) = f16x8{};      // what stands beside it in the planes
+  double s = 0.;
+#pragma unroll
+  for (int k = 0; k < 64; ++k) s = fma((double)g[k], (double)g[k], s);
   const float scale = (float)(SX / (sqrt(block_sum64(s, red)) + (double)p.eps));
-  for (int i = t; i < mp * np; i += 512) {        // the source's fast index is the thread's
-    const int fast = tall ? i % mp : i % np, slow = tall ? i / mp : i / np, r = tall ? fast : slow, c = tall ? slow : fast;
-    const float v = r < q.m && c < q.n ? ns_load(q, tall ? c : r, tall ? r : c) * scale : 0.f;
-    split16(v, Xh[r * ldx + c], Xl[r * ldx + c]);
+#pragma unroll
+  for (int k = 0; k < 64; ++k) {
+    const int e = t + 512 * k, r = row_of(e), c = e - r * q.cols, o = tall ? c * ldx + r : r * ldx + c;
+    if (e < total) split16(g[k] * scale, Xh[o], Xl[o]);
   }
   __syncthreads();
-  const int splits = ns_small_splits(mt), units = mt * mt * splits;
+  int lane = threadIdx.x & 63;
+#pragma unroll 1
   for (int step = 0; step < p.steps; ++step) {
-    f32x16 acc[4];
-    // A = X X^T: wave takes unit u = (tile, share of the columns)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int u = wave + 8 * j;
-      acc[j] = 0.f;
-      if (u >= units) continue;
-      const int tile = u / splits, sp = u % splits, ti = tile / mt, tj = tile % mt;
-      const int chunks = np / 16, per = (chunks + splits - 1) / splits;
-      for (int k = sp * per; k < min(chunks, (sp + 1) * per); ++k) {
-        const f16x8 ah = frag_k(Xh, ldx, ti * 32, k * 16, lane), al = frag_k(Xl, ldx, ti * 32, k * 16, lane);
-        const f16x8 bh = frag_k(Xh, ldx, tj * 32, k * 16, lane), bl = frag_k(Xl, ldx, tj * 32, k * 16, lane);
-        acc[j] = MFMA16(al, bh, acc[j]);
-        acc[j] = MFMA16(ah, bl, acc[j]);
-        acc[j] = MFMA16(ah, bh, acc[j]);
-      }
-      if (sp > 0) {
-        float* o = part + ((sp - 1) * mt * mt + tile) * 1024 + lane;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[r * 64] = acc[j][r];
-      }
-    }
-    if (splits > 1) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int u = wave + 8 * j;
-      if (u >= units || u % splits) continue;
-      const int tile = u / splits, ti = tile / mt, tj = tile % mt;
-      for (int sp = 1; sp < splits; ++sp) {
-        const float* o = part + ((sp - 1) * mt * mt + tile) * 1024 + lane;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[j][r] += o[r * 64];
-      }
+    asm volatile("" : "+v"(lane));       // else every address of the loop is kept in a register, and those in scratch
+    const int h = lane >> 5;
+    // A = X X^T: a wave takes (tile, share of the columns) units
+#pragma unroll 1
+    for (int u = wave; u < UNITS; u += 8) {
+      const int tile = u / SPLITS, sp = u % SPLITS, ti = tile / MT, tj = tile % MT;
+      const int chunks = np / 16, per = (chunks + SPLITS - 1) / SPLITS;
+      const f32x16 acc = small_tile<false>(Xh, Xl, ldx, ti * 32, Xh, Xl, ldx, tj * 32, min(chunks, sp * per) * 16,
+                                           min(chunks, (sp + 1) * per) * 16, lane);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int o = (ti * 32 + c_row(r, h)) * lda + tj * 32 + (lane & 31);
-        split16(acc[j][r] * (SA / (SX * SX)), Ah[o], Al[o]);
+        const int row = c_row(r, h), c = lane & 31;
+        if constexpr (SPLITS > 1) part[u * 1024 + row * 32 + c] = acc[r];
+        else {
+          const int o = (ti * 32 + row) * LDA + tj * 32 + c;
+          split16(acc[r] * (SA / (SX * SX)), Ah[o], Al[o]);
+        }
       }
     }
     __syncthreads();
-    // W = a I + b A + c A A into A's place
+    if constexpr (SPLITS > 1) {
+      for (int i = t; i < MT * MT * 1024; i += 512) {
+        const int tile = i >> 10, e = i & 1023;
+        float v = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int tile = wave + 8 * j;
-      if (tile >= mt * mt) continue;
-      const int ti = tile / mt, tj = tile % mt;
-      f32x16 sq = 0.f;
-      for (int k = 0; k < mp; k += 16) {
-        const f16x8 ah = frag_k(Ah, lda, ti * 32, k, lane), al = frag_k(Al, lda, ti * 32, k, lane);
-        const f16x8 bh = frag_k(Ah, lda, tj * 32, k, lane), bl = frag_k(Al, lda, tj * 32, k, lane);
-        sq = MFMA16(al, bh, sq);
-        sq = MFMA16(ah, bl, sq);
-        sq = MFMA16(ah, bh, sq);
+        for (int sp = 0; sp < SPLITS; ++sp) v += part[(tile * SPLITS + sp) * 1024 + e];
+        const int o = (tile / MT * 32 + (e >> 5)) * LDA + tile % MT * 32 + (e & 31);
+        split16(v * (SA / (SX * SX)), Ah[o], Al[o]);
       }
+      __syncthreads();
+    }
+    // W = a I + b A + c A A, into A's place once all have read it
+    f32x16 w[NA];
+#pragma unroll
+    for (int j = 0; j < NA; ++j) {
+      const int tile = wave + 8 * j;
+      if (tile >= MT * MT) continue;
+      const int ti = tile / MT, tj = tile % MT;
+      w[j] = small_tile<false>(Ah, Al, LDA, ti * 32, Ah, Al, LDA, tj * 32, 0, MP, lane);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = ti * 32 + c_row(r, h), c = tj * 32 + (lane & 31);
-        const float av = (float)Ah[row * lda + c] + (float)Al[row * lda + c];
-        acc[j][r] = p.b * av + (p.c / SA) * sq[r] + (row == c ? p.a * SA : 0.f);
+        const float av = (float)Ah[row * LDA + c] + (float)Al[row * LDA + c];
+        w[j][r] = p.b * av + (p.c / SA) * w[j][r] + (row == c ? p.a * SA : 0.f);
       }
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NA; ++j) {
       const int tile = wave + 8 * j;
-      if (tile >= mt * mt) continue;
-      const int ti = tile / mt, tj = tile % mt;
+      if (tile >= MT * MT) continue;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int o = (ti * 32 + c_row(r, h)) * lda + tj * 32 + (lane & 31);
-        split16(acc[j][r], Ah[o], Al[o]);
+        const int o = (tile / MT * 32 + c_row(r, h)) * LDA + tile % MT * 32 + (lane & 31);
+        split16(w[j][r], Ah[o], Al[o]);
       }
     }
     __syncthreads();
-    // X' = W X, up to four tiles a wave
+    // X' = W X, up to four tiles a wave, written once all have read X
+    f32x16 x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int tile = wave + 8 * j;
-      acc[j] = 0.f;
-      if (tile >= mt * nt) continue;
-      const int ti = tile / nt, tj = tile % nt;
-      for (int k = 0; k < mp; k += 16) {
-        const f16x8 ah = frag_kp(Ah, lda, ti * 32, k, lane), al = frag_kp(Al, lda, ti * 32, k, lane);
-        const f16x8 bh = frag_t(Xh, ldx, k, tj * 32, lane), bl = frag_t(Xl, ldx, k, tj * 32, lane);
-        acc[j] = MFMA16(al, bh, acc[j]);
-        acc[j] = MFMA16(ah, bl, acc[j]);
-        acc[j] = MFMA16(ah, bh, acc[j]);
-      }
+      if (tile < MT * nt) x[j] = small_tile<true>(Ah, Al, LDA, tile % MT * 32, Xh, Xl, ldx, tile / MT * 32, 0, MP, lane);
     }
     __syncthreads();
     const bool last = step + 1 == p.steps;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int tile = wave + 8 * j;
-      if (tile >= mt * nt) continue;
-      const int ti = tile / nt, tj = tile % nt;
+      if (tile >= MT * nt) continue;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = ti * 32 + c_row(r, h), c = tj * 32 + (lane & 31);
-        const float v = acc[j][r] * (1.f / SA);
+        const int row = tile % MT * 32 + c_row(r, h), c = tile / MT * 32 + (lane & 31);
+        const float v = x[j][r] * (1.f / SA);
         if (!last) split16(v, Xh[row * ldx + c], Xl[row * ldx + c]);
-        else if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, v * (1.f / SX));
+        else if (row < q.m && c < q.n) ((T*)q.dst)[tall ? (long)c * q.ld_dst + row : (long)row * q.ld_dst + c] = (T)(v * (1.f / SX));
       }
     }
     __syncthreads();
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512, 2) void ns_small(const NsSmallArgs p) {
+  extern __shared__ __align__(16) _Float16 lds[];
+  __shared__ double red[8];
+  const NsMat& q = p.mat[blockIdx.x];
+  switch (q.mp / 32) {
+    case 1: ns_small_run<T, 1>(p, q, lds, red); break;
+    case 2: ns_small_run<T, 2>(p, q, lds, red); break;
+    case 3: ns_small_run<T, 3>(p, q, lds, red); break;
+    default: ns_small_run<T, 4>(p, q, lds, red); break;
   }
 }
 
@@ -531,7 +579,7 @@ bool ns_large_dims(NsMat& q) {
   q.mp = cdiv(q.m, NS_TILE) * NS_TILE;
   q.np = cdiv(q.n, NS_TILE) * NS_TILE;
   const int nt = q.mp / NS_TILE, tiles = nt * (nt + 1) / 2;
-  q.splits = std::max(1, std::min(512 / tiles, q.np / NS_TILE));
+  q.splits = std::max(1, std::min(256 / tiles, q.np / NS_TILE));
   return true;
 }
 
@@ -564,7 +612,8 @@ bool ns_allow_lds() {
     return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n) == hipSuccess;
   };
   if (!allow((const void*)ns_gram, tile_lds) || !allow((const void*)ns_poly, tile_lds) ||
-      !allow((const void*)ns_apply, tile_lds) || !allow((const void*)ns_small, NS_SMALL_LDS))
+      !allow((const void*)ns_apply, tile_lds) || !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
+      !allow((const void*)ns_small<__bf16>, NS_SMALL_LDS) || !allow((const void*)ns_small<_Float16>, NS_SMALL_LDS))
     return false;
   done.fetch_or(bit);
   return true;
@@ -616,7 +665,9 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
   int ns = 0;
   size_t small_lds = 0;
   const auto flush_small = [&] {
-    if (ns) ns_small<<<ns, 512, small_lds, s>>>(small);
+    if (ns && type == TY_F32) ns_small<float><<<ns, 512, small_lds, s>>>(small);
+    else if (ns && type == TY_BF16) ns_small<__bf16><<<ns, 512, small_lds, s>>>(small);
+    else if (ns) ns_small<_Float16><<<ns, 512, small_lds, s>>>(small);
     ns = 0;
     small_lds = 0;
   };
