@@ -412,55 +412,56 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
   }
 }
 
-// joins the splits of a row: a workgroup takes 32 value columns of it, eight threads a column the splits in turn
-template <typename T, int D>
-__global__ __launch_bounds__(256) void da_join(const DaArgs a) {
-  constexpr int DV = 2 * D;
-  __shared__ float sh[2][8][32], red[4][8];
+// joins the splits of a row: a workgroup takes 32 value columns of it, GR threads a column the splits in turn; the splits'
+// factors are formed once, in LDS
+// (a thread each: at most 32 GR splits)
+template <typename T, int D, int GR>
+__global__ __launch_bounds__(32 * GR) void da_join(const DaArgs a) {
+  constexpr int DV = 2 * D, NW = GR / 2;
+  __shared__ float fac[2][32 * GR], sh[2][GR][33], red[4][NW];
   const long n = blockIdx.x;
   const int bh = (int)(n / a.R), r = (int)(n - (long)bh * a.R), b = bh / a.Hkv, hk = bh - b * a.Hkv, t = r / a.G,
             head = hk * a.G + r - t * a.G, col = threadIdx.x & 31, grp = threadIdx.x >> 5, c0 = blockIdx.y * 32 + col;
   const float* p = a.part + n * (2 * DV + 4);
   const long step = a.rows * (2 * DV + 4);
-  float m[2] = {-INFINITY, -INFINITY};
-  for (int s = threadIdx.x; s < a.splits; s += 256) {
-    m[0] = fmaxf(m[0], p[s * step + 2 * DV]);
-    m[1] = fmaxf(m[1], p[s * step + 2 * DV + 2]);
-  }
+  const int s0 = threadIdx.x;                      
+  f32x4 ml = {-INFINITY, 0.f, -INFINITY, 0.f};
+  if (s0 < a.splits) ml = *(const f32x4*)(p + s0 * step + 2 * DV);
+  float m[2], l[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    m[c] = wave_max(m[c]);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][c] = m[c];
+    m[c] = wave_max(ml[2 * c]);
+    if ((threadIdx.x & 63) == 0) red[c][threadIdx.x >> 6] = m[c];
   }
   __syncthreads();
 #pragma unroll
-  for (int c = 0; c < 2; ++c) m[c] = fmaxf(fmaxf(red[0][c], red[1][c]), fmaxf(red[2][c], red[3][c]));
-  float l[2] = {0.f, 0.f}, o[2] = {0.f, 0.f};
-#pragma unroll 4
-  for (int s = grp; s < a.splits; s += 8)
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float ms = p[s * step + 2 * DV + 2 * c];
-      const float f = ms == -INFINITY ? 0.f : ms == m[c] ? 1.f : exp2f((ms - m[c]) * a.c);
-      l[c] = fmaf(p[s * step + 2 * DV + 2 * c + 1], f, l[c]);
-      o[c] = fmaf(p[s * step + c * DV + c0], f, o[c]);
-    }
+    for (int w = 0; w < NW; ++w) m[c] = fmaxf(m[c], red[c][w]);
+    const float f = ml[2 * c] == -INFINITY ? 0.f : ml[2 * c] == m[c] ? 1.f : exp2f((ml[2 * c] - m[c]) * a.c);
+    if (s0 < a.splits) fac[c][s0] = f;
+    l[c] = wave_sum(ml[2 * c + 1] * f);
+    if ((threadIdx.x & 63) == 0) red[2 + c][threadIdx.x >> 6] = l[c];
+  }
+  __syncthreads();
+  float o[2] = {0.f, 0.f};
+#pragma unroll 8
+  for (int s = grp; s < a.splits; s += GR) {
+    o[0] = fmaf(p[s * step + c0], fac[0][s], o[0]);
+    o[1] = fmaf(p[s * step + DV + c0], fac[1][s], o[1]);
+  }
+  sh[0][grp][col] = o[0];
+  sh[1][grp][col] = o[1];
+  __syncthreads();
+  if (grp) return;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    __syncthreads();
-    sh[0][grp][col] = l[c];
-    sh[1][grp][col] = o[c];
-    __syncthreads();
-    if (grp == 0) {
-      l[c] = o[c] = 0.f;
+    l[c] = o[c] = 0.f;
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        l[c] += sh[0][g][col];
-        o[c] += sh[1][g][col];
-      }
-    }
+    for (int w = 0; w < NW; ++w) l[c] += red[2 + c][w];
+#pragma unroll
+    for (int g = 0; g < GR; ++g) o[c] += sh[c][g][col];
   }
-  if (grp) return;
   const float w = l[1] == 0.f ? 0.f : o[1] / l[1];
   const long out = ((long)(b * a.T + t) * a.H + head) * DV + c0;
   ((T*)a.o)[out] = (T)((l[0] == 0.f ? 0.f : o[0] / l[0]) - a.lam[head] * w);
@@ -871,12 +872,13 @@ __global__ __launch_bounds__(256) void da_kv_join(const DaArgs a) {
 // Two pairs of waves share a key tile where the rows fill them; a few rows over many keys are one pair.
 bool da_wide(long rows) { return rows > 32; }
 
-// Key splits that give every compute unit two workgroups of four waves, or four of two, with at least 128 keys each
+// Key splits that give every compute unit two workgroups of four waves, or of two as many as its LDS takes, with at least 128
+// keys each
 int da_splits(const ctr_diffattn_t* p) {
   const int R = p->T * (p->H / p->Hkv);
   const bool wide = da_wide(R);
   const long blocks = (long)cdiv(R, wide ? 64 : 32) * p->B * p->Hkv;
-  return (int)std::max<long>(1, std::min<long>((wide ? 512 : 1024) / std::max<long>(1, blocks), p->S / 128));
+  return (int)std::max<long>(1, std::min<long>((wide || p->D == 128 ? 512 : 1024) / std::max<long>(1, blocks), p->S / 128));
 }
 
 constexpr int da_pairs(int D) { return D == 128 ? 4 : 2; }
@@ -942,7 +944,8 @@ int da_run_fwd(DaArgs a, hipStream_t s) {
   const long blocks = a.tiles * bh * a.splits;
   if (wide) da_fwd<T, D, 2><<<(unsigned)blocks, 256, 0, s>>>(a);
   else da_fwd<T, D, 1><<<(unsigned)blocks, 128, 0, s>>>(a);
-  if (a.splits > 1) da_join<T, D><<<dim3((unsigned)a.rows, 2 * D / 32), 256, 0, s>>>(a);
+  if (a.splits > 32) da_join<T, D, 32><<<dim3((unsigned)a.rows, 2 * D / 32), 1024, 0, s>>>(a);
+  else if (a.splits > 1) da_join<T, D, 4><<<dim3((unsigned)a.rows, 2 * D / 32), 128, 0, s>>>(a);
   return check_launch("diffattn_fwd");
 }
 
