@@ -47,7 +47,7 @@ struct DaArgs {
 
 // Row statistics of the backward, written by the dQ kernel for the dK / dV kernel: a tile of 32 packed rows is 8 lines
 // of 32 words, one 1 KB load
-enum { RS_L1, RS_L2, RS_D1, RS_D2, RS_LAM, RS_LIM, RS_DL, RS_LINES = 8 };
+enum { RS_L1, RS_L2, RS_D1, RS_LD2, RS_LAM, RS_LIM, RS_DL, RS_LINES = 8 };      // RS_LD2: lam delta_2
 
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
@@ -93,48 +93,14 @@ __device__ __forceinline__ uint32_t col_base(const T* s, int lane) {
   const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)(s + row * W + ((c >> 3) ^ turn<W / 8>(row)) * 8 + (c & 4));
 }
-// Two column groups, 4 fragments.  The reads and their wait are one block: the compiler, which sees no address in the
-// transpose read, would wait for the next tile's loads before it.
+// columns 32 j .. of the panel's first (i = 0) or second 16 rows
 template <typename T, int W>
-__device__ __forceinline__ void frag_col2(uint32_t base, int j0, int j1, typename Vec<T>::v8 (&f)[2][2]) {
-  typedef typename Vec<T>::v4 v4;
-  const uint32_t p0 = base ^ (j0 << 6), p1 = base ^ (j1 << 6), q0 = (p0 + 16 * W) ^ 32, q1 = (p1 + 16 * W) ^ 32;
-  v4 a, b, c, d, e, g, h, i;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\t"
-      "ds_read_b64_tr_b16 %1, %9\n\t"
-      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %10\n\t"
-      "ds_read_b64_tr_b16 %5, %11\n\t"
-      "ds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(g), "=&v"(h), "=&v"(i)
-      : "v"(p0), "v"(q0), "v"(p1), "v"(q1), "n"(32 * W)
-      : "memory");
-  f[0][0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  f[0][1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
-  f[1][0] = __builtin_shufflevector(e, g, 0, 1, 2, 3, 4, 5, 6, 7);
-  f[1][1] = __builtin_shufflevector(h, i, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-// one column group
-template <typename T, int W>
-__device__ __forceinline__ void frag_col1(uint32_t base, typename Vec<T>::v8 (&f)[2]) {
-  typedef typename Vec<T>::v4 v4;
-  const uint32_t q0 = (base + 16 * W) ^ 32;
-  v4 a, b, c, d;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4\n\t"
-      "ds_read_b64_tr_b16 %1, %5\n\t"
-      "ds_read_b64_tr_b16 %2, %4 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
-      : "v"(base), "v"(q0), "n"(32 * W)
-      : "memory");
-  f[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  f[1] = __builtin_shufflevector(c, d, 0, 1, 2, 3, 4, 5, 6, 7);
+__device__ __forceinline__ typename Vec<T>::v8 frag_col(uint32_t base, int i, int j) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const uint32_t p = (base ^ (j << 6)) + i * 32 * W, q = ((base ^ (j << 6)) + 16 * W ^ 32) + i * 32 * W;
+  const auto u = __builtin_bit_cast(typename Vec<T>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+  const auto v = __builtin_bit_cast(typename Vec<T>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q));
+  return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 // registers 8 i .. 8 i + 7 of a C tile as an operand, and what the rounding left out
 template <typename T>
@@ -161,8 +127,6 @@ __device__ __forceinline__ typename Vec<T>::v8 pack_rest(const f32x16& v, typena
   }
   return __builtin_convertvector(o, typename Vec<T>::v8);
 }
-
-typedef __attribute__((address_space(3))) void lds_void;
 
 // Direct loads of a tile of 32 rows to LDS: two panels of width D (the maps) and one of 2 D (values, or dO), as four
 // roles dealt over the waves: panel 0, panel 1, the upper and the lower 16 rows of panel 2.  Each role is PER loads of
@@ -194,8 +158,11 @@ struct Stage {
   }
 };
 
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds, 16, off, 0, 0, 0);
+// 64 lanes x 16 bytes from r at off to consecutive LDS places.  Nothing comes back in registers, and tile_ready() waits: as a
+// builtin it would have the compiler wait for it before any transpose read, whose address it does not see.
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, const void* lds, uint32_t off) {
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory");
 }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t open_range(const void* p) { return buf_rsrc(p, 0x7ffffff0u); }
 
@@ -263,6 +230,7 @@ struct Seq {
 template <typename T, int D, int RG>
 __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da_fwd(const DaArgs a) {
   constexpr int DV = 2 * D, KQ = D / 16, NO = DV / 32, NW = 2 * RG, TILE = Stage<T, D, NW>::TILE;
+  constexpr int JG = NO < 4 ? NO : 4;
   static_assert(RG * DV * 32 * sizeof(float) <= 2 * TILE * sizeof(T), "the maps meet in the tiles' place");
   typedef typename Vec<T>::v8 v8;
   __shared__ __align__(1024) T tiles[2][TILE];
@@ -334,17 +302,17 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
     }
     const uint32_t vc = vcol + cur * TILE * sizeof(T);
 #pragma unroll
-    for (int j = 0; j < NO; j += 2) {
-      v8 vf[2][2];
-      frag_col2<T, DV>(vc, j, j + 1, vf);
+    for (int j0 = 0; j0 < NO; j0 += JG)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {        // no two products in a row into one accumulator
+        v8 vf[JG];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          o[j + e] = Mfma<T>::run(vf[e][i], pr[i], o[j + e]);
-          o[j + e] = Mfma<T>::run(vf[e][i], pf[i], o[j + e]);
-        }
-    }
+        for (int j = 0; j < JG; ++j) vf[j] = frag_col<T, DV>(vc, i, j0 + j);
+#pragma unroll
+        for (int j = 0; j < JG; ++j) o[j0 + j] = Mfma<T>::run(vf[j], pr[i], o[j0 + j]);
+#pragma unroll
+        for (int j = 0; j < JG; ++j) o[j0 + j] = Mfma<T>::run(vf[j], pf[i], o[j0 + j]);
+      }
   }
   l += __shfl_xor(l, 32, 64);
   const long n = (long)bh * a.R + row;
@@ -501,25 +469,10 @@ struct DsScale {
 template <typename T, int W, int N>
 __device__ __forceinline__ void add_cols(uint32_t base, const typename Vec<T>::v8 (&x)[2], f32x16 (&acc)[N]) {
   static_assert(N == W / 32, "panel");
-  if constexpr (N == 1 || N == 8) {       // eight tiles leave no registers for two groups
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      typename Vec<T>::v8 f[2];
-      frag_col1<T, W>(base ^ (j << 6), f);
-      acc[j] = Mfma<T>::run(f[0], x[0], acc[j]);
-      acc[j] = Mfma<T>::run(f[1], x[1], acc[j]);
-    }
-  } else {
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      typename Vec<T>::v8 f[2][2];
-      frag_col2<T, W>(base, j, j + 1, f);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) acc[j + e] = Mfma<T>::run(f[e][i], x[i], acc[j + e]);
-    }
-  }
+    for (int j = 0; j < N; ++j) acc[j] = Mfma<T>::run(frag_col<T, W>(base, i, j), x[i], acc[j]);
 }
 
 // dQ: a wave owns 32 rows, walks the keys; also the rows' statistics for the dK / dV kernel
@@ -579,14 +532,14 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
     const T* ks = tiles[cur];
     const T* vs = ks + 64 * D;
     f32x16 sc[2], dp = 0.f;
+    sc[0] = sc[1] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      sc[c] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KQ; ++k) sc[c] = Mfma<T>::run(frag_row<T, D>(ks + c * 32 * D, k, lane), qf[c][k], sc[c]);
+    for (int k = 0; k < KQ; ++k) {         // three accumulators in turn
+      sc[0] = Mfma<T>::run(frag_row<T, D>(ks, k, lane), qf[0][k], sc[0]);
+      dp = Mfma<T>::run(frag_row<T, DV>(vs, 2 * k, lane), gf[2 * k], dp);
+      sc[1] = Mfma<T>::run(frag_row<T, D>(ks + 32 * D, k, lane), qf[1][k], sc[1]);
+      dp = Mfma<T>::run(frag_row<T, DV>(vs, 2 * k + 1, lane), gf[2 * k + 1], dp);
     }
-#pragma unroll
-    for (int k = 0; k < KV; ++k) dp = Mfma<T>::run(frag_row<T, DV>(vs, k, lane), gf[k], dp);
     const int end = lim - kb;
     const bool edge = __any(end < 32);
 #pragma unroll
@@ -630,7 +583,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
     rs[32 * RS_L1] = on && lim ? l1 : INFINITY;
     rs[32 * RS_L2] = on && lim ? l2 : INFINITY;
     rs[32 * RS_D1] = on ? d1 : 0.f;
-    rs[32 * RS_D2] = on ? d2 : 0.f;
+    rs[32 * RS_LD2] = on ? lam * d2 : 0.f;
     rs[32 * RS_LAM] = on ? lam : 0.f;
     rs[32 * RS_LIM] = __builtin_bit_cast(float, on ? lim : 0);
     rs[32 * RS_DL] = on ? dl : 0.f;
@@ -679,7 +632,7 @@ __global__ __launch_bounds__(1024) void da_dlam(const DaArgs a) { head_dlam(a, b
 // dP, dS and dK_c = dS_c^T Q_c; the probabilities pass from one to the other through LDS in fp32, once a tile.  Each so
 // holds half of the accumulators and two waves fit a SIMD: one's exponentials run under the other's products.
 template <typename T, int D, int NP>
-__global__ __launch_bounds__(128 * NP, 2) void da_bwd_kv(const DaArgs a) {
+__global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const DaArgs a) {
   constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32, NW = 2 * NP, TILE = Stage<T, D, NW>::TILE;
   constexpr bool HALF = DsScale<T>::ON;
   constexpr float PS = HALF ? 1024.f : 1.f;       // |P_1 - lam P_2| <= max(1, |lam|): keeps fp16's P out of the subnormals
@@ -703,8 +656,12 @@ __global__ __launch_bounds__(128 * NP, 2) void da_bwd_kv(const DaArgs a) {
     r0 += sp * per;
     r1 = min(r1, r0 + per);
   }
+  // row rb is position tb, head `rem`; rb moves by 32.  A row's position from there is a division of a number below G + 32
+  // by G: the upper half of its product with ceil(2^32 / G), exact below 2^16.
+  int tb = r0 / a.G, rem = r0 - tb * a.G;
+  const uint32_t magic = a.G == 1 ? 0 : (uint32_t)((0x100000000ull + a.G - 1) / a.G);
+  const auto over_g = [&](int n) { return a.G == 1 ? n : (int)__umulhi((uint32_t)n, magic); };
   const auto stage = [&](int rb, int cur) {
-    const int tb = rb / a.G;
     const auto qb = (const T*)a.q + s.b * a.q_sb + tb * a.q_st + s.hk * a.G * a.q_sh;
     const auto gb = (const T*)a.dout + s.b * a.g_sb + tb * a.g_st + s.hk * a.G * a.g_sh;
 #pragma unroll
@@ -714,10 +671,15 @@ __global__ __launch_bounds__(128 * NP, 2) void da_bwd_kv(const DaArgs a) {
       const int st = (int)((role < 2 ? a.q_st : a.g_st) * sizeof(T)), sh = (int)((role < 2 ? a.q_sh : a.g_sh) * sizeof(T));
 #pragma unroll
       for (int j = 0; j < St::PER; ++j) {
-        const int r = rb + plan.row[i] + j * step, t = r / a.G, g = r - t * a.G;
-        dma16(rs, tiles[cur] + St::place(role, wave) + j * 512, r < r1 ? (t - tb) * st + g * sh + plan.byte[i][j] : BUF_OOB);
+        const int x = plan.row[i] + j * step, t = over_g(rem + x), g = rem + x - t * a.G;
+        const uint32_t off = t * st + g * sh + plan.byte[i][j];
+        dma16(rs, tiles[cur] + St::place(role, wave) + j * 512, rb + x < r1 ? off : BUF_OOB);
       }
     }
+    rem += 32;
+    const int t = over_g(rem);
+    tb += t;
+    rem -= t * a.G;
     if (wave == 0) dma16(open_range(a.part + ((long)bh * a.tiles32 + rb / 32) * (RS_LINES * 32)), stats[cur], lane * 16);
   };
   if (r0 < r1) stage(r0, 0);
@@ -747,29 +709,44 @@ __global__ __launch_bounds__(128 * NP, 2) void da_bwd_kv(const DaArgs a) {
       const float* st = stats[cur];
       // a row below the diagonal of the pair's last key, or a key behind the end, needs the mask
       const bool edge = kw + 32 > s.kl || (a.causal && rb / a.G + s.kl - s.ql < kw + 31);
-      f32x16 pc;
+      f32x16 pc, sc[2];
+      sc[0] = sc[1] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        f32x16 sc = 0.f;
+      for (int k = 0; k < KQ; ++k) {
+        sc[0] = Mfma<T>::run(frag_row<T, D>(qs, k, lane), kf[0][k], sc[0]);
+        sc[1] = Mfma<T>::run(frag_row<T, D>(qs + 32 * D, k, lane), kf[1][k], sc[1]);
+      }
 #pragma unroll
-        for (int k = 0; k < KQ; ++k) sc = Mfma<T>::run(frag_row<T, D>(qs + c * 32 * D, k, lane), kf[c][k], sc);
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int at = 8 * r4 + 4 * h;
-          const f32x4 ls = *(const f32x4*)(st + 32 * (c ? RS_L2 : RS_L1) + at);
+          const f32x4 ls = *(const f32x4*)(st + 32 * (c ? RS_L2 : RS_L1) + 8 * r4 + 4 * h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[c][4 * r4 + j] = __builtin_amdgcn_exp2f(fmaf(sc[c][4 * r4 + j], a.c, -ls[j]));
+        }
+      if (edge) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const i32x4 lim = *(const i32x4*)(st + 32 * RS_LIM + 8 * r4 + 4 * h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[0][4 * r4 + j] = key < lim[j] ? sc[0][4 * r4 + j] : 0.f;
+            sc[1][4 * r4 + j] = key < lim[j] ? sc[1][4 * r4 + j] : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4 lam = *(const f32x4*)(st + 32 * RS_LAM + 8 * r4 + 4 * h);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
           f32x4 p;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(sc[4 * r4 + j], a.c, -ls[j]));
-          if (c) p *= *(const f32x4*)(st + 32 * RS_LAM + at);
-          if (edge) {
-            const i32x4 lim = *(const i32x4*)(st + 32 * RS_LIM + at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = key < lim[j] ? p[j] : 0.f;
-          }
+          for (int j = 0; j < 4; ++j) p[j] = sc[c][4 * r4 + j];
           probs[pair][c][r4][lane] = p;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) pc[4 * r4 + j] = c ? pc[4 * r4 + j] - p[j] : p[j];
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pc[4 * r4 + j] = fmaf(-lam[j], sc[1][4 * r4 + j], sc[0][4 * r4 + j]);
       }
       if constexpr (HALF) pc *= PS;
       const v8 pf[2] = {pack<T>(pc, 0), pack<T>(pc, 1)};
@@ -816,13 +793,14 @@ __global__ __launch_bounds__(128 * NP, 2) void da_bwd_kv(const DaArgs a) {
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int at = 8 * r4 + 4 * h;
-        const f32x4 d1 = *(const f32x4*)(st + 32 * RS_D1 + at), d2 = *(const f32x4*)(st + 32 * RS_D2 + at);
+        const f32x4 d1 = *(const f32x4*)(st + 32 * RS_D1 + at), d2 = *(const f32x4*)(st + 32 * RS_LD2 + at),
+                    lam = *(const f32x4*)(st + 32 * RS_LAM + at);
         const f32x4 p1 = probs[pair][0][r4][lane], p2 = probs[pair][1][r4][lane];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * r4 + j;
           ds[0][r] = p1[j] * (dp[r] - d1[j]);
-          ds[1][r] = p2[j] * (d2[j] - dp[r]);
+          ds[1][r] = p2[j] * fmaf(-lam[j], dp[r], d2[j]);
         }
       }
       const float down = fit.fit(ds[0], ds[1]);
@@ -898,7 +876,7 @@ int da_check(const ctr_diffattn_t* p, bool bwd) {
   CTR_REQUIRE(p->type == TY_BF16 || p->type == TY_F16, "type (1 bf16, 2 fp16)");
   CTR_REQUIRE(p->D == 32 || p->D == 64 || p->D == 128, "map width D in {32, 64, 128}");
   CTR_REQUIRE(p->B >= 0 && p->T >= 0 && p->S >= 0 && p->H >= 1 && p->Hkv >= 1 && p->H % p->Hkv == 0, "sizes");
-  CTR_REQUIRE((long)p->T * (p->H / p->Hkv) < (1L << 30) && p->S < (1 << 30), "sizes");
+  CTR_REQUIRE((long)p->T * (p->H / p->Hkv) < (1L << 30) && p->S < (1 << 30) && p->H / p->Hkv < (1 << 15), "sizes");
   CTR_REQUIRE((long)p->B * p->Hkv * cdiv((long)p->T * (p->H / p->Hkv), 32) < (1L << 31) &&
                   (long)p->B * p->Hkv * cdiv(p->S, 32) < (1L << 31) && (long)p->B * p->H * p->T < (1L << 31), "sizes");
   CTR_REQUIRE(p->scale > 0.f && std::isfinite(p->scale), "scale > 0");
