@@ -22,9 +22,7 @@ namespace {
 constexpr float SX = 4096.f, SA = 1024.f;      // the planes' scales of X and of A, W
 constexpr int NS_MAXMAT = 20;                  // matrices of one launch (their table rides in the kernel arguments)
 constexpr int NS_TILE = 128, NS_BK = 32;
-constexpr int LDK = NS_BK + 8, LDN = NS_TILE + 32;   // LDS row strides (elements): k-contiguous tiles, n-contiguous tiles
-constexpr int PLANE_K = NS_TILE * LDK, PLANE_N = NS_BK * LDN;
-static_assert(PLANE_K == PLANE_N, "one LDS plane size");
+constexpr int NS_STAGE = 4 * NS_TILE * NS_BK;        // elements of a K step in LDS: two planes of either operand
 constexpr int NS_SUMSQ_BLOCKS = 256;
 constexpr int NS_SMALL_LDS = 160 * 1024 - 256;   // of a workgroup, next to its few static bytes
 
@@ -34,8 +32,8 @@ struct NsMat {
   long ld_src, ld_dst;
   int rows, cols;          // as given
   int m, n, mp, np;        // m <= n, and both rounded up to the tile
-  long off_x, off_a, off_p, off_s;     // bytes into the workspace: X planes (two buffers), A / W planes, Gram partials, sums
-  int splits, type;
+  long off_x, off_a, off_p, off_s;     // bytes into the workspace: X planes (two buffers), A and W planes, partials, sums
+  int splits, asplits, type;           // shares of K of X X^T and of A A
 };
 struct NsArgs {
   int count;
@@ -162,68 +160,91 @@ __global__ __launch_bounds__(256) void ns_init(const NsArgs p) {
   }
 }
 
+// 64 lanes x 16 bytes to consecutive LDS places.  Nothing comes back in registers and the K loop waits for it by count.
+__device__ __forceinline__ void ns_dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t off, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void ns_wait() {      // all but the last N loads have landed, in every wave
+  static_assert(N <= 63, "vmcnt");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // One 128 x 128 tile of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.
-// Four waves of 64 x 64; the next step's tiles are loaded to registers under this step's products.
-template <bool NN>
+// Four waves of 64 x 64.  A K step's four planes (wave w loads plane w) come by direct loads to one of NST places in LDS,
+// NST - 1 steps ahead: two places and two workgroups a compute unit where there are enough tiles, four and one where a
+// tile's chain of steps is what counts.  Rows of 64 bytes (k) hold their 16-byte chunk c at c ^ (row / 4 % 4), rows of 256
+// bytes (columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads then cover all banks.
+template <bool NN, int NST>
 __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda, const _Float16* B, long planeB, int ldb,
                                         int r0, int c0, int k0, int k1, _Float16* lds, f32x16 acc[2][2]) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
-  f16x8 ra[4], rb[4];
-  const auto fetch = [&](int k) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
+  const bool cols = NN && wave >= 2;
+  const int ld = wave < 2 ? lda : ldb;
+  const _Float16* src = wave < 2 ? A + (wave & 1) * planeA + (long)r0 * lda + k0
+                                 : B + (wave & 1) * planeB + (NN ? (long)k0 * ldb + c0 : (long)c0 * ldb + k0);
+  uint32_t off[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int id = t + (j & 1) * 256;
-      ra[j] = *(const f16x8*)(A + (j >> 1) * planeA + (long)(r0 + id / 4) * lda + k + id % 4 * 8);
-      rb[j] = NN ? *(const f16x8*)(B + (j >> 1) * planeB + (long)(k + id / 16) * ldb + c0 + id % 16 * 8)
-                 : *(const f16x8*)(B + (j >> 1) * planeB + (long)(c0 + id / 4) * ldb + k + id % 4 * 8);
-    }
-  };
-  const auto put = [&](_Float16* s) {
+  for (int j = 0; j < 4; ++j)
+    off[j] = cols ? (lane >> 4) * ld * 2 + (((lane & 15) ^ ((lane >> 4) << 2)) ^ j) * 16 : (lane >> 2) * ld * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
+  const uint32_t jump = (cols ? 4 : 16) * ld * 2;
+  const auto stage = [&](int step, int place) {
+    const auto rs = buf_rsrc(src + (long)step * NS_BK * (cols ? ldb : 1), 0x7ffffff0u);
+    const uint32_t to = lds0 + (place * NS_STAGE + wave * NS_TILE * NS_BK) * 2;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int id = t + (j & 1) * 256;
-      *(f16x8*)(s + (j >> 1) * PLANE_K + id / 4 * LDK + id % 4 * 8) = ra[j];
-      if (NN) *(f16x8*)(s + (2 + (j >> 1)) * PLANE_K + id / 16 * LDN + id % 16 * 8) = rb[j];
-      else *(f16x8*)(s + (2 + (j >> 1)) * PLANE_K + id / 4 * LDK + id % 4 * 8) = rb[j];
-    }
+    for (int j = 0; j < 8; ++j) ns_dma16(rs, to + j * 1024, off[j & 3], j * jump);
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = 0.f;
-  if (k0 >= k1) return;
-  fetch(k0);
-  put(lds);
-  __syncthreads();
-  int cur = 0;
-  for (int k = k0; k < k1; k += NS_BK) {
-    const bool more = k + NS_BK < k1;
-    if (more) fetch(k + NS_BK);
-    const _Float16* s = lds + cur * 4 * PLANE_K;
+  const int steps = (k1 - k0) / NS_BK;
 #pragma unroll
-    for (int kk = 0; kk < NS_BK; kk += 16) {
+  for (int i = 0; i < NST - 1; ++i)
+    if (i < steps) stage(i, i);
+  const int row = lane & 31, h = lane >> 5;
+  const int arow = (wr + row) * NS_BK, brow = (wc + row) * NS_BK, turn = (row >> 2) & 3;
+  const int tk = 8 * h + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;      // transpose reads: row, column
+  int place = 0;
+  for (int k = 0; k < steps; ++k) {
+    if (k + NST - 1 <= steps) ns_wait<8 * (NST - 2)>();
+    else ns_wait<0>();
+    if (k + NST - 1 < steps) stage(k + NST - 1, place == 0 ? NST - 1 : place - 1);
+    const _Float16* s = lds + place * NS_STAGE;
+    place = place + 1 == NST ? 0 : place + 1;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
       f16x8 a[2][2], b[2][2];      // [plane][tile]
+      const int ch = ((2 * kk + h) ^ turn) * 8;
 #pragma unroll
       for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          a[pl][i] = NN ? frag_kp(s + pl * PLANE_K, LDK, wr + 32 * i, kk, lane)
-                        : frag_k(s + pl * PLANE_K, LDK, wr + 32 * i, kk, lane);
-          b[pl][i] = NN ? frag_t(s + (2 + pl) * PLANE_K, LDN, kk, wc + 32 * i, lane)
-                        : frag_k(s + (2 + pl) * PLANE_K, LDK, wc + 32 * i, kk, lane);
+          a[pl][i] = *(const f16x8*)(s + pl * NS_TILE * NS_BK + arow + 32 * i * NS_BK + ch);
+          const _Float16* bp = s + (2 + pl) * NS_TILE * NS_BK;
+          if constexpr (!NN) b[pl][i] = *(const f16x8*)(bp + brow + 32 * i * NS_BK + ch);
+          else {
+            f16x4 u[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int r = 16 * kk + tk + 4 * half, c = wc + 32 * i + tc;
+              const _Float16* q = bp + r * NS_TILE + ((c >> 3) ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (c & 4);
+              u[half] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
+            }
+            b[pl][i] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          }
         }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int pr = 0; pr < 3; ++pr)      // lo hi, hi lo, hi hi; four accumulators in turn
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[i][j] = MFMA16(a[1][i], b[0][j], acc[i][j]);
-          acc[i][j] = MFMA16(a[0][i], b[1][j], acc[i][j]);
-          acc[i][j] = MFMA16(a[0][i], b[0][j], acc[i][j]);
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = MFMA16(a[pr == 0][i], b[pr == 1][j], acc[i][j]);
     }
-    if (more) put(lds + (cur ^ 1) * 4 * PLANE_K);
-    __syncthreads();
-    cur ^= 1;
   }
 }
 
@@ -235,20 +256,22 @@ __device__ __forceinline__ void tri(int id, int& ti, int& tj) {
   tj = id - ti * (ti + 1) / 2;
 }
 
-// Gram partials: A = X X^T over a share of the columns, lower tiles
-__global__ __launch_bounds__(256, 2) void ns_gram(const NsArgs p, int buf) {
+// partials of X X^T (square = false) or A A over a share of K, lower tiles; the workgroups of an XCD (every eighth) take the
+// same share, whose rows so stay in its L2
+template <int NST>
+__global__ __launch_bounds__(256, NST == 2 ? 2 : 1) void ns_gram(const NsArgs p, int buf, bool square) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
-  const int id = blockIdx.x - p.pre[i], nt = q.mp / NS_TILE, tiles = nt * (nt + 1) / 2, sp = id / tiles;
+  const int splits = square ? q.asplits : q.splits, id = blockIdx.x - p.pre[i], sp = id % splits, K = square ? q.mp : q.np;
   int ti, tj;
-  tri(id % tiles, ti, tj);
-  const int steps = q.np / NS_BK, per = (steps + q.splits - 1) / q.splits;
-  const long plane = (long)q.mp * q.np;
-  const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
+  tri(id / splits, ti, tj);
+  const int steps = K / NS_BK, per = (steps + splits - 1) / splits;
+  const long plane = (long)q.mp * K;
+  const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
   f32x16 acc[2][2];
-  ns_tile<false>(x, plane, q.np, x, plane, q.np, ti * NS_TILE, tj * NS_TILE, min(steps, sp * per) * NS_BK,
-                 min(steps, (sp + 1) * per) * NS_BK, lds, acc);
+  ns_tile<false, NST>(x, plane, K, x, plane, K, ti * NS_TILE, tj * NS_TILE, min(steps, sp * per) * NS_BK,
+                      min(steps, (sp + 1) * per) * NS_BK, lds, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -261,29 +284,40 @@ __global__ __launch_bounds__(256, 2) void ns_gram(const NsArgs p, int buf) {
             b * 32 + (lane & 31)] = acc[a][b][r];
 }
 
-// the partials of a 32 x 32 block of the lower tiles summed in order (four elements a thread, eight loads in flight), both
-// triangles' planes written
-__global__ __launch_bounds__(256) void ns_gram_join(const NsArgs p) {
+// the partials of a 32 x 32 block of the lower tiles summed in order (four elements a thread, eight loads in flight), and A
+// (square = false) or W = a I + b A + c A A written, both triangles' planes
+__global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
   __shared__ float tile[32][33];
   int ti, tj;
   tri(blockIdx.x - p.pre[i], ti, tj);
-  _Float16* A = (_Float16*)(p.ws + q.off_a);
   const long plane = (long)q.mp * q.mp;
+  const _Float16* A = (const _Float16*)(p.ws + q.off_a);
+  _Float16* out = (_Float16*)(p.ws + q.off_a) + (square ? 2 * plane : 0);
+  const int splits = square ? q.asplits : q.splits;
   const int r = threadIdx.x >> 3, c4 = (threadIdx.x & 7) * 4;
   const float* in = (const float*)(p.ws + q.off_p) + (long)(ti * 32 + r) * q.mp + tj * 32 + c4;
   f32x4 v = 0.f;
   int s = 0;
-  for (; s + 8 <= q.splits; s += 8) {
+  for (; s + 8 <= splits; s += 8) {
     f32x4 u[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) u[k] = *(const f32x4*)(in + (s + k) * plane);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v += u[k];
   }
-  for (; s < q.splits; ++s) v += *(const f32x4*)(in + s * plane);
-  v *= SA / (SX * SX);
+  for (; s < splits; ++s) v += *(const f32x4*)(in + s * plane);
+  if (square) {
+    const long o = (long)(ti * 32 + r) * q.mp + tj * 32 + c4;
+    const f32x4 av = __builtin_convertvector(*(const f16x4*)(A + o), f32x4) + __builtin_convertvector(*(const f16x4*)(A + plane + o), f32x4);
+    v = p.b * av + (p.c / SA) * v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (ti * 32 + r == tj * 32 + c4 + k) v[k] += p.a * SA;
+  } else {
+    v *= SA / (SX * SX);
+  }
   const auto put = [&](int row, int col, const f32x4& x) {
     f16x4 hi, lo;
 #pragma unroll
@@ -293,8 +327,8 @@ __global__ __launch_bounds__(256) void ns_gram_join(const NsArgs p) {
       hi[k] = a;
       lo[k] = b;
     }
-    *(f16x4*)(A + (long)row * q.mp + col) = hi;
-    *(f16x4*)(A + plane + (long)row * q.mp + col) = lo;
+    *(f16x4*)(out + (long)row * q.mp + col) = hi;
+    *(f16x4*)(out + plane + (long)row * q.mp + col) = lo;
   };
   put(ti * 32 + r, tj * 32 + c4, v);
   if (ti == tj) return;      // the whole block: it is symmetric by itself
@@ -306,61 +340,21 @@ __global__ __launch_bounds__(256) void ns_gram_join(const NsArgs p) {
   put(tj * 32 + r, ti * 32 + c4, v);
 }
 
-// W = a I + b A + c A A, lower tiles, both triangles written
-__global__ __launch_bounds__(256, 2) void ns_poly(const NsArgs p) {
+// X' = W X; the last step writes the result in its own type and orientation.  An XCD takes every eighth panel of columns, with
+// all row tiles of one together.
+template <int NST>
+__global__ __launch_bounds__(256, NST == 2 ? 2 : 1) void ns_apply(const NsArgs p, int buf, int last) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
-  int ti, tj;
-  tri(blockIdx.x - p.pre[i], ti, tj);
-  const long plane = (long)q.mp * q.mp;
-  const _Float16* A = (const _Float16*)(p.ws + q.off_a);
-  _Float16* Wp = (_Float16*)(p.ws + q.off_a) + 2 * plane;
-  f32x16 acc[2][2];
-  ns_tile<false>(A, plane, q.mp, A, plane, q.mp, ti * NS_TILE, tj * NS_TILE, 0, q.mp, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int c = tj * NS_TILE + (wave & 1) * 64 + b * 32 + (lane & 31);
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        f16x4 hi, lo;
-        const int row0 = ti * NS_TILE + (wave >> 1) * 64 + a * 32 + c_row(4 * r4, lane >> 5);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const long o = (long)(row0 + r) * q.mp + c;
-          float v = p.b * ((float)A[o] + (float)A[plane + o]) + (p.c / SA) * acc[a][b][4 * r4 + r];
-          if (row0 + r == c) v += p.a * SA;
-          _Float16 h, l;
-          split16(v, h, l);
-          hi[r] = h;
-          lo[r] = l;
-          Wp[o] = h;
-          Wp[plane + o] = l;
-        }
-        if (ti != tj) {
-          const long o = (long)c * q.mp + row0;
-          *(f16x4*)(Wp + o) = hi;
-          *(f16x4*)(Wp + plane + o) = lo;
-        }
-      }
-    }
-}
-
-// X' = W X; the last step writes the result in its own type and orientation
-__global__ __launch_bounds__(256, 2) void ns_apply(const NsArgs p, int buf, int last) {
-  extern __shared__ __align__(16) _Float16 lds[];
-  const int i = ns_find(p, blockIdx.x);
-  const NsMat& q = p.mat[i];
-  const int id = blockIdx.x - p.pre[i], mt = q.mp / NS_TILE, r0 = id % mt * NS_TILE, c0 = id / mt * NS_TILE;
+  const int id = blockIdx.x - p.pre[i], mt = q.mp / NS_TILE, r0 = (id >> 3) % mt * NS_TILE, c0 = ((id >> 3) / mt * 8 + (id & 7)) * NS_TILE;
+  if (c0 >= q.np) return;
   const long plane = (long)q.mp * q.np, planeW = (long)q.mp * q.mp;
   const _Float16* W = (const _Float16*)(p.ws + q.off_a) + 2 * planeW;
   const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
   _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
   f32x16 acc[2][2];
-  ns_tile<true>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
+  ns_tile<true, NST>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool tall = q.rows > q.cols;
 #pragma unroll
@@ -554,7 +548,7 @@ size_t ns_layout(NsMat& q, size_t off) {
   const auto take = [&](size_t n) { const size_t o = off; off = (off + n + 255) / 256 * 256; return (long)o; };
   q.off_x = take((size_t)8 * q.mp * q.np);         // two buffers of two planes
   q.off_a = take((size_t)8 * q.mp * q.mp);         // A and W
-  q.off_p = take((size_t)4 * q.splits * q.mp * q.mp);
+  q.off_p = take((size_t)4 * std::max(q.splits, q.asplits) * q.mp * q.mp);
   q.off_s = take((size_t)8 * NS_SUMSQ_BLOCKS);
   return off;
 }
@@ -574,12 +568,27 @@ void ns_dims(NsMat& q, const ctr_ns_mat_t& g, int type) {
   q.np = cdiv(q.n, 32) * 32;
 }
 
+// Shares of K of a symmetric product: those whose workgroups come nearest to filling the 512 places of the card (two a compute
+// unit) a whole number of times, each with at least four K steps; a share costs its partial sums, written and read once.
+int ns_splits(int tiles, int K) {
+  const int most = std::max(1, std::min({K / (4 * NS_BK), std::max(1, 256 / tiles), 32}));
+  if (tiles < 32) return most;
+  int best = 1;
+  double cost = 1e30;
+  for (int s = 1; s <= std::max(1, std::min(8, K / (4 * NS_BK))); ++s) {
+    const double c = (double)cdiv((long)tiles * s, 512) / s + 0.01 * s;
+    if (c < cost) cost = c, best = s;
+  }
+  return best;
+}
+
 bool ns_large_dims(NsMat& q) {
   if (ns_is_small(q.mp, q.np)) return false;
   q.mp = cdiv(q.m, NS_TILE) * NS_TILE;
   q.np = cdiv(q.n, NS_TILE) * NS_TILE;
   const int nt = q.mp / NS_TILE, tiles = nt * (nt + 1) / 2;
-  q.splits = std::max(1, std::min(256 / tiles, q.np / NS_TILE));
+  q.splits = ns_splits(tiles, q.np);
+  q.asplits = ns_splits(tiles, q.mp);
   return true;
 }
 
@@ -600,6 +609,8 @@ bool ns_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
+constexpr int ns_lds(int nst) { return nst * NS_STAGE * (int)sizeof(_Float16); }
+
 // the kernels' LDS beyond 64 KB, once for each device
 bool ns_allow_lds() {
   static std::atomic<uint64_t> done{0};
@@ -607,12 +618,11 @@ bool ns_allow_lds() {
   if (hipGetDevice(&dev) != hipSuccess) return false;
   const uint64_t bit = 1ull << (dev & 63);
   if (done.load() & bit) return true;
-  const int tile_lds = 8 * PLANE_K * (int)sizeof(_Float16);
   const auto allow = [](const void* f, int n) {
     return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n) == hipSuccess;
   };
-  if (!allow((const void*)ns_gram, tile_lds) || !allow((const void*)ns_poly, tile_lds) ||
-      !allow((const void*)ns_apply, tile_lds) || !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
+  if (!allow((const void*)ns_gram<2>, ns_lds(2)) || !allow((const void*)ns_gram<4>, ns_lds(4)) ||
+      !allow((const void*)ns_apply<2>, ns_lds(2)) || !allow((const void*)ns_apply<4>, ns_lds(4)) || !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
       !allow((const void*)ns_small<__bf16>, NS_SMALL_LDS) || !allow((const void*)ns_small<_Float16>, NS_SMALL_LDS))
     return false;
   done.fetch_or(bit);
@@ -689,20 +699,21 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
   };
   const auto flush_large = [&] {
     if (large.count == 0) return;
-    const size_t lds = 8 * PLANE_K * sizeof(_Float16);
+    const auto tri_n = [](int n) { return n * (n + 1) / 2; };
     ns_sumsq<<<dim3(NS_SUMSQ_BLOCKS, large.count), 256, 0, s>>>(large);
     const int ni = prefix([](const NsMat& q) { return q.mp / 64 * (q.np / 64); });
     ns_init<<<ni, 256, 0, s>>>(large);
     for (int k = 0; k < steps; ++k) {
-      const auto tri_n = [](int n) { return n * (n + 1) / 2; };
-      const int ng = prefix([&](const NsMat& q) { return q.splits * tri_n(q.mp / NS_TILE); });
-      ns_gram<<<ng, 256, lds, s>>>(large, k & 1);
-      const int nj = prefix([&](const NsMat& q) { return tri_n(q.mp / 32); });
-      ns_gram_join<<<nj, 256, 0, s>>>(large);
-      const int np = prefix([&](const NsMat& q) { return tri_n(q.mp / NS_TILE); });
-      ns_poly<<<np, 256, lds, s>>>(large);
-      const int na = prefix([](const NsMat& q) { return q.mp / NS_TILE * (q.np / NS_TILE); });
-      ns_apply<<<na, 256, lds, s>>>(large, k & 1, k + 1 == steps);
+      for (int square = 0; square < 2; ++square) {
+        const int ng = prefix([&](const NsMat& q) { return (square ? q.asplits : q.splits) * tri_n(q.mp / NS_TILE); });
+        if (ng > 256) ns_gram<2><<<ng, 256, ns_lds(2), s>>>(large, k & 1, square);
+        else ns_gram<4><<<ng, 256, ns_lds(4), s>>>(large, k & 1, square);
+        const int nj = prefix([&](const NsMat& q) { return tri_n(q.mp / 32); });
+        ns_join<<<nj, 256, 0, s>>>(large, square);
+      }
+      const int na = prefix([](const NsMat& q) { return q.mp / NS_TILE * (cdiv(q.np / NS_TILE, 8) * 8); });
+      if (na > 256) ns_apply<2><<<na, 256, ns_lds(2), s>>>(large, k & 1, k + 1 == steps);
+      else ns_apply<4><<<na, 256, ns_lds(4), s>>>(large, k & 1, k + 1 == steps);
     }
     large.count = 0;
     off = 0;
