@@ -22,7 +22,6 @@ namespace {
 constexpr float SX = 4096.f, SA = 1024.f;      // the planes' scales of X and of A, W
 constexpr int NS_MAXMAT = 20;                  // matrices of one launch (their table rides in the kernel arguments)
 constexpr int NS_TILE = 128, NS_BK = 32;
-constexpr int NS_STAGE = 4 * NS_TILE * NS_BK;        // elements of a K step in LDS: two planes of either operand
 constexpr int NS_SUMSQ_BLOCKS = 256;
 constexpr int NS_SMALL_LDS = 160 * 1024 - 256;   // of a workgroup, next to its few static bytes
 
@@ -33,7 +32,8 @@ struct NsMat {
   int rows, cols;          // as given
   int m, n, mp, np;        // m <= n, and both rounded up to the tile
   long off_x, off_a, off_p, off_s;     // bytes into the workspace: X planes (two buffers), A and W planes, partials, sums
-  int splits, asplits, type;           // shares of K of X X^T and of A A
+  int splits, asplits, type, wr;      // shares of K of X X^T and of A A; the tile rows in 64s
+ 
 };
 struct NsArgs {
   int count;
@@ -173,30 +173,37 @@ __device__ __forceinline__ void ns_wait() {      // all but the last N loads hav
   asm volatile("" ::: "memory");
 }
 
-// One 128 x 128 tile of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.
-// Four waves of 64 x 64.  A K step's four planes (wave w loads plane w) come by direct loads to one of NST places in LDS,
-// NST - 1 steps ahead: two places and two workgroups a compute unit where there are enough tiles, four and one where a
-// tile's chain of steps is what counts.  Rows of 64 bytes (k) hold their 16-byte chunk c at c ^ (row / 4 % 4), rows of 256
-// bytes (columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads then cover all banks.
-template <bool NN, int NST>
+// A tile of 64 WR x 128 of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.
+// 2 WR waves of 64 x 64.  A K step's four planes come by direct loads to one of NST places in LDS, NST - 1 steps ahead:
+// eight waves (WR = 4) and three places where there are tiles for every compute unit -- the step's products last shorter
+// than a load, so one step ahead is not enough, and the larger tile reads a quarter less --, four waves and four places
+// where a tile's chain of steps is what counts.  Rows of 64 bytes (k) hold their 16-byte chunk c at c ^ (row / 4 % 4), rows
+// of 256 bytes (columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads then cover all banks.
+template <int WR> constexpr int ns_stage() { return 2 * NS_BK * (64 * WR + NS_TILE); }      // elements of a step's planes
+template <bool NN, int WR, int NST>
 __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda, const _Float16* B, long planeB, int ldb,
                                         int r0, int c0, int k0, int k1, _Float16* lds, f32x16 acc[2][2]) {
+  constexpr int PA = 64 * WR * NS_BK, PB = NS_TILE * NS_BK, STAGE = ns_stage<WR>(), NB = 8 / WR, LOADS = 4 + NB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
-  const bool cols = NN && wave >= 2;
-  const int ld = wave < 2 ? lda : ldb;
-  const _Float16* src = wave < 2 ? A + (wave & 1) * planeA + (long)r0 * lda + k0
-                                 : B + (wave & 1) * planeB + (NN ? (long)k0 * ldb + c0 : (long)c0 * ldb + k0);
-  uint32_t off[4];
+  // wave w loads of plane w / WR the A rows 64 (w % WR) .., and that share of the B rows or K rows
+  const int pl = wave / WR, sh = wave % WR;
+  const _Float16* asrc = A + pl * planeA + (long)(r0 + 64 * sh) * lda + k0;
+  const _Float16* bsrc = B + pl * planeB + (NN ? (long)(k0 + NS_BK / WR * sh) * ldb + c0 : (long)(c0 + NS_TILE / WR * sh) * ldb + k0);
+  const uint32_t aoff = (lane >> 2) * lda * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
+  uint32_t boff[NB];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    off[j] = cols ? (lane >> 4) * ld * 2 + (((lane & 15) ^ ((lane >> 4) << 2)) ^ j) * 16 : (lane >> 2) * ld * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
-  const uint32_t jump = (cols ? 4 : 16) * ld * 2;
+  for (int j = 0; j < NB; ++j)
+    boff[j] = NN ? (lane >> 4) * ldb * 2 + (((lane & 15) ^ ((lane >> 4) << 2)) ^ ((NB * sh + j) & 3)) * 16
+                 : (lane >> 2) * ldb * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
   const auto stage = [&](int step, int place) {
-    const auto rs = buf_rsrc(src + (long)step * NS_BK * (cols ? ldb : 1), 0x7ffffff0u);
-    const uint32_t to = lds0 + (place * NS_STAGE + wave * NS_TILE * NS_BK) * 2;
+    const auto ra = buf_rsrc(asrc + (long)step * NS_BK, 0x7ffffff0u);
+    const auto rb = buf_rsrc(bsrc + (long)step * NS_BK * (NN ? ldb : 1), 0x7ffffff0u);
+    const uint32_t ta = lds0 + (place * STAGE + pl * PA + sh * 64 * NS_BK) * 2, tb = lds0 + (place * STAGE + 2 * PA + pl * PB + sh * (PB / WR)) * 2;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ns_dma16(rs, to + j * 1024, off[j & 3], j * jump);
+    for (int j = 0; j < 4; ++j) ns_dma16(ra, ta + j * 1024, aoff, j * 32 * lda);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) ns_dma16(rb, tb + j * 1024, boff[j], j * (NN ? 8 : 32) * ldb);
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -211,10 +218,10 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda,
   const int tk = 8 * h + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;      // transpose reads: row, column
   int place = 0;
   for (int k = 0; k < steps; ++k) {
-    if (k + NST - 1 <= steps) ns_wait<8 * (NST - 2)>();
+    if (k + NST - 1 <= steps) ns_wait<LOADS * (NST - 2)>();
     else ns_wait<0>();
     if (k + NST - 1 < steps) stage(k + NST - 1, place == 0 ? NST - 1 : place - 1);
-    const _Float16* s = lds + place * NS_STAGE;
+    const _Float16* s = lds + place * STAGE;
     place = place + 1 == NST ? 0 : place + 1;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -224,8 +231,8 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda,
       for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          a[pl][i] = *(const f16x8*)(s + pl * NS_TILE * NS_BK + arow + 32 * i * NS_BK + ch);
-          const _Float16* bp = s + (2 + pl) * NS_TILE * NS_BK;
+          a[pl][i] = *(const f16x8*)(s + pl * PA + arow + 32 * i * NS_BK + ch);
+          const _Float16* bp = s + 2 * PA + pl * PB;
           if constexpr (!NN) b[pl][i] = *(const f16x8*)(bp + brow + 32 * i * NS_BK + ch);
           else {
             f16x4 u[2];
@@ -256,21 +263,37 @@ __device__ __forceinline__ void tri(int id, int& ti, int& tj) {
   tj = id - ti * (ti + 1) / 2;
 }
 
+// tiles of 64 WR x 128 that meet the lower triangle, row by row
+template <int WR>
+__device__ __forceinline__ void tri_tile(int id, int& ti, int& tj) {
+  if constexpr (WR == 2) tri(id, ti, tj);
+  else {
+    tri(id >> 1, ti, tj);       // row ti has 2 (ti + 1) of them
+    tj = 2 * tj + (id & 1);
+  }
+}
+__host__ __device__ inline int tri_tiles(int mp, int wr) {
+  const int n = mp / (64 * wr);
+  return n * (n + 1) / 2 * (wr == 2 ? 1 : 2);
+}
+
 // partials of X X^T (square = false) or A A over a share of K, lower tiles; the workgroups of an XCD (every eighth) take the
 // same share, whose rows so stay in its L2
-template <int NST>
-__global__ __launch_bounds__(256, NST == 2 ? 2 : 1) void ns_gram(const NsArgs p, int buf, bool square) {
+template <int WR, int NST>
+__global__ __launch_bounds__(128 * WR, 1) void ns_gram(const NsArgs p, int buf, bool square) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
-  const int splits = square ? q.asplits : q.splits, id = blockIdx.x - p.pre[i], sp = id % splits, K = square ? q.mp : q.np;
+  const int splits = square ? q.asplits : q.splits, id = blockIdx.x - p.pre[i], K = square ? q.mp : q.np;
+  const int tiles = tri_tiles(q.mp, WR), sp = (id >> 3) / tiles * 8 + (id & 7);
+  if (sp >= splits) return;
   int ti, tj;
-  tri(id / splits, ti, tj);
+  tri_tile<WR>((id >> 3) % tiles, ti, tj);
   const int steps = K / NS_BK, per = (steps + splits - 1) / splits;
   const long plane = (long)q.mp * K;
   const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
   f32x16 acc[2][2];
-  ns_tile<false, NST>(x, plane, K, x, plane, K, ti * NS_TILE, tj * NS_TILE, min(steps, sp * per) * NS_BK,
+  ns_tile<false, WR, NST>(x, plane, K, x, plane, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
                       min(steps, (sp + 1) * per) * NS_BK, lds, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -280,7 +303,7 @@ __global__ __launch_bounds__(256, NST == 2 ? 2 : 1) void ns_gram(const NsArgs p,
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        out[(long)(ti * NS_TILE + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * NS_TILE + (wave & 1) * 64 +
+        out[(long)(ti * 64 * WR + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * NS_TILE + (wave & 1) * 64 +
             b * 32 + (lane & 31)] = acc[a][b][r];
 }
 
@@ -342,38 +365,54 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
 
 // X' = W X; the last step writes the result in its own type and orientation.  An XCD takes every eighth panel of columns, with
 // all row tiles of one together.
-template <int NST>
-__global__ __launch_bounds__(256, NST == 2 ? 2 : 1) void ns_apply(const NsArgs p, int buf, int last) {
+template <int WR, int NST>
+__global__ __launch_bounds__(128 * WR, 1) void ns_apply(const NsArgs p, int buf, int last) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
-  const int id = blockIdx.x - p.pre[i], mt = q.mp / NS_TILE, r0 = (id >> 3) % mt * NS_TILE, c0 = ((id >> 3) / mt * 8 + (id & 7)) * NS_TILE;
+  const int id = blockIdx.x - p.pre[i], mt = q.mp / (64 * WR), r0 = (id >> 3) % mt * 64 * WR, c0 = ((id >> 3) / mt * 8 + (id & 7)) * NS_TILE;
   if (c0 >= q.np) return;
   const long plane = (long)q.mp * q.np, planeW = (long)q.mp * q.mp;
   const _Float16* W = (const _Float16*)(p.ws + q.off_a) + 2 * planeW;
   const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
   _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
   f32x16 acc[2][2];
-  ns_tile<true, NST>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
+  ns_tile<true, WR, NST>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool tall = q.rows > q.cols;
+  if (last) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int c = c0 + (wave & 1) * 64 + b * 32 + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = r0 + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5);
+          if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, acc[a][b][r] * (1.f / (SA * SX)));
+        }
+      }
+    return;
+  }
+  // the planes go out through LDS, 16 bytes a lane along a row
+  constexpr int LD = NS_TILE + 8, PL = 64 * WR * LD;
+  __syncthreads();
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int c = c0 + (wave & 1) * 64 + b * 32 + (lane & 31);
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = r0 + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5);
-        const float v = acc[a][b][r] * (1.f / SA);
-        if (last) {
-          if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, v * (1.f / SX));
-        } else {
-          const long o = (long)row * q.np + c;
-          split16(v, y[o], y[plane + o]);
-        }
+        const int o = ((wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5)) * LD + (wave & 1) * 64 + b * 32 + (lane & 31);
+        split16(acc[a][b][r] * (1.f / SA), lds[o], lds[PL + o]);
       }
-    }
+  __syncthreads();
+  constexpr int PER = 2 * 64 * WR * (NS_TILE / 8) / (128 * WR);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int e = threadIdx.x + k * 128 * WR, c = e % (NS_TILE / 8), row = e / (NS_TILE / 8) % (64 * WR), pl = e / (NS_TILE / 8) / (64 * WR);
+    *(f16x8*)(y + pl * plane + (long)(r0 + row) * q.np + c0 + c * 8) = *(const f16x8*)(lds + pl * PL + row * LD + c * 8);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -568,15 +607,14 @@ void ns_dims(NsMat& q, const ctr_ns_mat_t& g, int type) {
   q.np = cdiv(q.n, 32) * 32;
 }
 
-// Shares of K of a symmetric product: those whose workgroups come nearest to filling the 512 places of the card (two a compute
-// unit) a whole number of times, each with at least four K steps; a share costs its partial sums, written and read once.
+// Shares of K of a symmetric product: as many as give every compute unit a workgroup, a whole number of times as nearly as may
+// be, each with at least four K steps; a share costs its partial sums, written and read once.
 int ns_splits(int tiles, int K) {
-  const int most = std::max(1, std::min({K / (4 * NS_BK), std::max(1, 256 / tiles), 32}));
-  if (tiles < 32) return most;
+  const int most = std::max(1, std::min(K / (4 * NS_BK), 32));
   int best = 1;
   double cost = 1e30;
-  for (int s = 1; s <= std::max(1, std::min(8, K / (4 * NS_BK))); ++s) {
-    const double c = (double)cdiv((long)tiles * s, 512) / s + 0.01 * s;
+  for (int s = 1; s <= most; ++s) {
+    const double c = (double)cdiv((long)tiles * s, 256) / s * 256. / tiles + 0.02 * s;
     if (c < cost) cost = c, best = s;
   }
   return best;
@@ -584,9 +622,11 @@ int ns_splits(int tiles, int K) {
 
 bool ns_large_dims(NsMat& q) {
   if (ns_is_small(q.mp, q.np)) return false;
-  q.mp = cdiv(q.m, NS_TILE) * NS_TILE;
+  q.wr = q.m > 768 ? 4 : 2;
+  q.mp = cdiv(q.m, 64 * q.wr) * 64 * q.wr;
   q.np = cdiv(q.n, NS_TILE) * NS_TILE;
-  const int nt = q.mp / NS_TILE, tiles = nt * (nt + 1) / 2;
+  if (q.np < q.mp) q.np = q.mp;
+  const int tiles = tri_tiles(q.mp, q.wr);
   q.splits = ns_splits(tiles, q.np);
   q.asplits = ns_splits(tiles, q.mp);
   return true;
@@ -609,7 +649,8 @@ bool ns_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
-constexpr int ns_lds(int nst) { return nst * NS_STAGE * (int)sizeof(_Float16); }
+constexpr int NS_LDS4 = 3 * ns_stage<4>() * (int)sizeof(_Float16), NS_LDS2 = 4 * ns_stage<2>() * (int)sizeof(_Float16);
+static_assert(2 * 256 * (NS_TILE + 8) * 2 <= NS_LDS4 && 2 * 128 * (NS_TILE + 8) * 2 <= NS_LDS2, "the result's planes take the K steps' place");
 
 // the kernels' LDS beyond 64 KB, once for each device
 bool ns_allow_lds() {
@@ -621,8 +662,9 @@ bool ns_allow_lds() {
   const auto allow = [](const void* f, int n) {
     return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n) == hipSuccess;
   };
-  if (!allow((const void*)ns_gram<2>, ns_lds(2)) || !allow((const void*)ns_gram<4>, ns_lds(4)) ||
-      !allow((const void*)ns_apply<2>, ns_lds(2)) || !allow((const void*)ns_apply<4>, ns_lds(4)) || !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
+  if (!allow((const void*)ns_gram<4, 3>, NS_LDS4) || !allow((const void*)ns_gram<2, 4>, NS_LDS2) ||
+      !allow((const void*)ns_apply<4, 3>, NS_LDS4) || !allow((const void*)ns_apply<2, 4>, NS_LDS2) ||
+      !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
       !allow((const void*)ns_small<__bf16>, NS_SMALL_LDS) || !allow((const void*)ns_small<_Float16>, NS_SMALL_LDS))
     return false;
   done.fetch_or(bit);
@@ -635,17 +677,18 @@ bool ns_allow_lds() {
 using namespace ctr;
 
 extern "C" size_t ctr_newton_schulz_ws_size(const ctr_ns_mat_t* mats, int count) {
-  size_t most = 0, off = 0;
-  int in = 0;
+  size_t most = 0, off[2] = {0, 0};
+  int in[2] = {0, 0};
   for (int i = 0; mats && i < count; ++i) {
     if (mats[i].rows <= 0 || mats[i].cols <= 0) continue;
     NsMat q;
     ns_dims(q, mats[i], 0);
     if (!ns_large_dims(q)) continue;
-    if (in == NS_MAXMAT) in = 0, off = 0;
-    off = ns_layout(q, off);
-    ++in;
-    most = std::max(most, off);
+    const int g = q.wr == 4;
+    if (in[g] == NS_MAXMAT) in[g] = 0, off[g] = 0;
+    off[g] = ns_layout(q, off[g]);
+    ++in[g];
+    most = std::max(most, off[g]);
   }
   return most;
 }
@@ -681,51 +724,54 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     ns = 0;
     small_lds = 0;
   };
-  NsArgs large = {};
-  large.ws = (char*)ws;
-  large.a = a;
-  large.b = b;
-  large.c = c;
-  large.eps = eps;
-  size_t off = 0;
-  const auto prefix = [&](auto blocks) {
-    int n = 0;
-    for (int i = 0; i < large.count; ++i) {
-      large.pre[i] = n;
-      n += blocks(large.mat[i]);
-    }
-    large.pre[large.count] = n;
-    return n;
-  };
-  const auto flush_large = [&] {
-    if (large.count == 0) return;
-    const auto tri_n = [](int n) { return n * (n + 1) / 2; };
-    ns_sumsq<<<dim3(NS_SUMSQ_BLOCKS, large.count), 256, 0, s>>>(large);
+  NsArgs large[2] = {};             // by their tile
+  size_t off[2] = {0, 0};
+  for (NsArgs& g : large) {
+    g.ws = (char*)ws;
+    g.a = a;
+    g.b = b;
+    g.c = c;
+    g.eps = eps;
+  }
+  const auto flush_large = [&](int w) {
+    NsArgs& g = large[w];
+    if (g.count == 0) return;
+    const auto prefix = [&](auto blocks) {
+      int n = 0;
+      for (int i = 0; i < g.count; ++i) {
+        g.pre[i] = n;
+        n += blocks(g.mat[i]);
+      }
+      g.pre[g.count] = n;
+      return n;
+    };
+    ns_sumsq<<<dim3(NS_SUMSQ_BLOCKS, g.count), 256, 0, s>>>(g);
     const int ni = prefix([](const NsMat& q) { return q.mp / 64 * (q.np / 64); });
-    ns_init<<<ni, 256, 0, s>>>(large);
+    ns_init<<<ni, 256, 0, s>>>(g);
     for (int k = 0; k < steps; ++k) {
       for (int square = 0; square < 2; ++square) {
-        const int ng = prefix([&](const NsMat& q) { return (square ? q.asplits : q.splits) * tri_n(q.mp / NS_TILE); });
-        if (ng > 256) ns_gram<2><<<ng, 256, ns_lds(2), s>>>(large, k & 1, square);
-        else ns_gram<4><<<ng, 256, ns_lds(4), s>>>(large, k & 1, square);
-        const int nj = prefix([&](const NsMat& q) { return tri_n(q.mp / 32); });
-        ns_join<<<nj, 256, 0, s>>>(large, square);
+        const int ng = prefix([&](const NsMat& q) { return cdiv(square ? q.asplits : q.splits, 8) * 8 * tri_tiles(q.mp, q.wr); });
+        if (w) ns_gram<4, 3><<<ng, 512, NS_LDS4, s>>>(g, k & 1, square);
+        else ns_gram<2, 4><<<ng, 256, NS_LDS2, s>>>(g, k & 1, square);
+        const int nj = prefix([](const NsMat& q) { return (q.mp / 32) * (q.mp / 32 + 1) / 2; });
+        ns_join<<<nj, 256, 0, s>>>(g, square);
       }
-      const int na = prefix([](const NsMat& q) { return q.mp / NS_TILE * (cdiv(q.np / NS_TILE, 8) * 8); });
-      if (na > 256) ns_apply<2><<<na, 256, ns_lds(2), s>>>(large, k & 1, k + 1 == steps);
-      else ns_apply<4><<<na, 256, ns_lds(4), s>>>(large, k & 1, k + 1 == steps);
+      const int na = prefix([](const NsMat& q) { return q.mp / (64 * q.wr) * (cdiv(q.np / NS_TILE, 8) * 8); });
+      if (w) ns_apply<4, 3><<<na, 512, NS_LDS4, s>>>(g, k & 1, k + 1 == steps);
+      else ns_apply<2, 4><<<na, 256, NS_LDS2, s>>>(g, k & 1, k + 1 == steps);
     }
-    large.count = 0;
-    off = 0;
+    g.count = 0;
+    off[w] = 0;
   };
   for (int i = 0; i < count; ++i) {
     if (mats[i].rows == 0 || mats[i].cols == 0) continue;
     NsMat q;
     ns_dims(q, mats[i], type);
     if (ns_large_dims(q)) {
-      if (large.count == NS_MAXMAT) flush_large();
-      off = ns_layout(q, off);
-      large.mat[large.count++] = q;
+      const int w = q.wr == 4;
+      if (large[w].count == NS_MAXMAT) flush_large(w);
+      off[w] = ns_layout(q, off[w]);
+      large[w].mat[large[w].count++] = q;
     } else {
       if (ns == NS_MAXMAT) flush_small();
       small_lds = std::max(small_lds, ns_small_lds(q.mp, q.np));
@@ -733,6 +779,7 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     }
   }
   flush_small();
-  flush_large();
+  flush_large(0);
+  flush_large(1);
   return check_launch("newton_schulz");
 }
