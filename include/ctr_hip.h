@@ -685,13 +685,14 @@ int ctr_ln_bwd(const void* dy, long lddy, const void* x, long ldx, const float* 
  * head serves H / Hkv consecutive query heads).  o (B, T, H, 2 D) contiguous.  q_lens / kv_lens (B) nullable: valid
  * positions and keys of each sequence, held to [0, T] / [0, S]; what stands behind
  * kv_lens does not count.  causal: position t sees the keys up to t + kv_len - q_len.  A row that sees no key, and a position behind q_len, gives zeros (and zero
- * gradients).  For the backward pass o2 (the shape of o: the second map's part) and stat (2 * B * H * T floats: the
- * rows' log-sums) are written by the forward; both null: inference.
+ * gradients).  For the backward pass o2 and ol (the shape and type of o: the second map's
+ * part, and what o's rounding left out) and stat (2 * B * H * T floats: the rows' log-sums) are written by the forward; all null:
+ * inference.
  * ctr_diffattn_bwd: dout (B, T, H, 2 D) with strides; dq, dk, dv contiguous in the shapes of q, k, v; dlam (H) fp32.  */
 typedef struct {
   const void *q, *k, *v;
   const float* lam;
-  void *o, *o2;
+  void *o, *o2, *ol;
   float* stat;
   const int32_t *q_lens, *kv_lens;
   long q_sb, q_st, q_sh, q_sc, k_sb, k_ss, k_sh, k_sc, v_sb, v_ss, v_sh;

@@ -75,7 +75,7 @@ def test_ln_entry_refusals():
 
 def attn(**kw):
     a = _lib.DiffAttn()
-    for f in ("q", "k", "v", "lam", "o", "o2", "stat"):
+    for f in ("q", "k", "v", "lam", "o", "o2", "ol", "stat"):
         setattr(a, f, P)
     B, T, S, H, Hkv, D = 2, 64, 64, 4, 2, 64
     a.q_sb, a.q_st, a.q_sh, a.q_sc = T * H * 2 * D, H * 2 * D, 2 * D, D
@@ -111,7 +111,7 @@ def test_diffattn_entry_workspaces_and_gradients():
     refuse("dout", "ctr_diffattn_bwd", *good(st=4))
     refuse("null operand", "ctr_diffattn_bwd", *good(dk=None))
     refuse("16-byte", "ctr_diffattn_bwd", *good(dq=P + 2))
-    b = attn(o2=None)
+    b = attn(o2=None, ol=None)
     refuse("null operand", "ctr_diffattn_bwd", C.byref(b), *good()[1:])
     assert _lib.call("ctr_diffattn_fwd", C.byref(attn(B=0)), None, 0, None) == 0
 

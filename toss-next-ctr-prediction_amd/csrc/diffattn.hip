@@ -19,7 +19,8 @@
 // accumulators and dlam's sum are fp32.
 // Roundings to 16 bits.  The forward's P enter the product with V as two 16-bit terms each (the value and what that leaves
 // out): O is a difference, and where the maps agree one rounding of either would be larger than the result's own.  In
-// the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.
+// the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.  What
+// the rounding of O left out is kept too: delta_1, taken from the rounded O alone, would add as much again to dQ of short rows.
 #include <algorithm>
 #include <atomic>
 
@@ -32,7 +33,7 @@ namespace {
 struct DaArgs {
   const void *q, *k, *v, *dout;
   const float* lam;
-  void *o, *o2;                  // (B, T, H, 2 D); o2 = P_2 V, kept for the backward (may be null)
+  void *o, *o2, *ol;             // (B, T, H, 2 D); kept for the backward (may be null): o2 = P_2 V, ol = what o's rounding left out
   float* stat;                   // 2 planes of rows: log2 sums of the maps
   void *dq, *dk, *dv;
   float* dlam;
@@ -374,6 +375,11 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = o[j][4 * r4 + r] * inv - lam * meet[(32 * j + c_row(4 * r4 + r, h)) * 32];
         put((T*)a.o + at, j, r4, x);
+        if (a.ol) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] -= (float)(T)x[r];
+          put((T*)a.ol + at, j, r4, x);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);       // one tile's reads at a time: the accumulators fill the registers
     }
@@ -432,8 +438,12 @@ __global__ __launch_bounds__(32 * GR) void da_join(const DaArgs a) {
   }
   const float w = l[1] == 0.f ? 0.f : o[1] / l[1];
   const long out = ((long)(b * a.T + t) * a.H + head) * DV + c0;
-  ((T*)a.o)[out] = (T)((l[0] == 0.f ? 0.f : o[0] / l[0]) - a.lam[head] * w);
-  if (a.o2) ((T*)a.o2)[out] = (T)w;
+  const float u = (l[0] == 0.f ? 0.f : o[0] / l[0]) - a.lam[head] * w;
+  ((T*)a.o)[out] = (T)u;
+  if (a.o2) {
+    ((T*)a.o2)[out] = (T)w;
+    ((T*)a.ol)[out] = (T)(u - (float)(T)u);
+  }
   if (a.stat && blockIdx.y == 0 && col < 2) {
     const float ll = col ? l[1] : l[0], mm = col ? m[1] : m[0];
     a.stat[col * a.rows + n] = ll == 0.f ? INFINITY : fmaf(mm, a.c, log2f(ll));
@@ -505,10 +515,11 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
     gf[k] = *(const v8*)(gp + 16 * k + 8 * h);
-    const v8 o = *(const v8*)((const T*)a.o + orow + 16 * k + 8 * h), o2 = *(const v8*)((const T*)a.o2 + orow + 16 * k + 8 * h);
+    const long at = orow + 16 * k + 8 * h;
+    const v8 o = *(const v8*)((const T*)a.o + at), o2 = *(const v8*)((const T*)a.o2 + at), ol = *(const v8*)((const T*)a.ol + at);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      d1 = fmaf((float)gf[k][i], (float)o[i], d1);
+      d1 = fmaf((float)gf[k][i], (float)o[i] + (float)ol[i], d1);
       d2 = fmaf((float)gf[k][i], (float)o2[i], d2);
     }
   }
@@ -558,8 +569,10 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
         dp[r] = seen ? dp[r] : 0.f;
       }
     }
+    float dl_tile = 0.f;              // a tile's sum by itself: long rows then add few numbers
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dl += dp[r];
+    for (int r = 0; r < 16; ++r) dl_tile += dp[r];
+    dl += dl_tile;
     const float down = fit.fit(sc[0], sc[1]);
     if (down != 1.f) {
 #pragma unroll
@@ -893,14 +906,14 @@ int da_check(const ctr_diffattn_t* p, bool bwd) {
   CTR_REQUIRE((long)p->B * p->T == 0 || ok(p->q, {p->q_sb, p->q_st, p->q_sh, p->q_sc}, p->q_st, G > 1 ? p->q_sh * std::min(32L, G) / 16 : 0), "q: 16-byte aligned rows");
   CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->k, {p->k_sb, p->k_ss, p->k_sh, p->k_sc}, p->k_ss, 0), "k: 16-byte aligned rows");
   CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->v, {p->v_sb, p->v_ss, p->v_sh}, p->v_ss, 0), "v: 16-byte aligned rows");
-  CTR_REQUIRE((long)p->B * p->T == 0 || (p->o && (uintptr_t)p->o % 16 == 0 && (uintptr_t)p->o2 % 16 == 0), "output");
+  CTR_REQUIRE((long)p->B * p->T == 0 || (p->o && (uintptr_t)p->o % 16 == 0 && (uintptr_t)p->o2 % 16 == 0 && (uintptr_t)p->ol % 16 == 0 && !p->o2 == !p->ol), "output");
   return 0;
 }
 
 DaArgs da_args(const ctr_diffattn_t* p) {
   DaArgs a = {};
   a.q = p->q; a.k = p->k; a.v = p->v; a.lam = p->lam;
-  a.o = p->o; a.o2 = p->o2; a.stat = p->stat;
+  a.o = p->o; a.o2 = p->o2; a.ol = p->ol; a.stat = p->stat;
   a.q_lens = p->q_lens; a.kv_lens = p->kv_lens;
   a.q_sb = p->q_sb; a.q_st = p->q_st; a.q_sh = p->q_sh; a.q_sc = p->q_sc;
   a.k_sb = p->k_sb; a.k_ss = p->k_ss; a.k_sh = p->k_sh; a.k_sc = p->k_sc;
@@ -992,7 +1005,7 @@ extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long 
   if (const int rc = da_check(p, true)) return rc;
   CTR_REQUIRE(dlam, "null dlam");
   const bool q_on = (long)p->B * p->T > 0, k_on = (long)p->B * p->S > 0;
-  CTR_REQUIRE(!q_on || (p->o2 && p->stat && dq && dout), "null operand");
+  CTR_REQUIRE(!q_on || (p->o2 && p->ol && p->stat && dq && dout), "null operand");
   CTR_REQUIRE(!q_on || ((uintptr_t)dout % 16 == 0 && g_sb % 8 == 0 && g_st % 8 == 0 && g_sh % 8 == 0 && g_sb >= 0 &&
                         g_st >= 0 && g_sh >= 0 && g_st < (1L << 24) && g_sh * (p->H / p->Hkv > 1) < (1L << 24)), "dout: 16-byte aligned rows");
   CTR_REQUIRE(!k_on || (dk && dv), "null operand");

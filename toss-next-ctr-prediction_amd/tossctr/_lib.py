@@ -51,7 +51,7 @@ class Seg(C.Structure):
 
 
 class DiffAttn(C.Structure):
-    _fields_ = [("q", p), ("k", p), ("v", p), ("lam", p), ("o", p), ("o2", p), ("stat", p), ("q_lens", p),
+    _fields_ = [("q", p), ("k", p), ("v", p), ("lam", p), ("o", p), ("o2", p), ("ol", p), ("stat", p), ("q_lens", p),
                 ("kv_lens", p), ("q_sb", l), ("q_st", l), ("q_sh", l), ("q_sc", l), ("k_sb", l), ("k_ss", l),
                 ("k_sh", l), ("k_sc", l), ("v_sb", l), ("v_ss", l), ("v_sh", l), ("scale", f), ("B", i), ("T", i),
                 ("S", i), ("H", i), ("Hkv", i), ("D", i), ("causal", i), ("type", i)]

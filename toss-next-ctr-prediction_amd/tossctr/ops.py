@@ -229,10 +229,10 @@ def diff_attention_fwd(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_l
     saved = None
     a.o = out.data_ptr()
     if save:
-        o2 = torch.empty_like(out)
+        parts = torch.empty((2, *out.shape), dtype=q.dtype, device=q.device)     # the second map's, out's remainder
         stat = torch.empty((2, a.B * a.H * a.T), dtype=torch.float32, device=q.device)
-        a.o2, a.stat = o2.data_ptr(), stat.data_ptr()
-        saved = (o2, stat)
+        a.o2, a.ol, a.stat = parts.data_ptr(), parts.data_ptr() + 2 * out.numel(), stat.data_ptr()
+        saved = (parts, stat)
     if out.numel():
         with _On(q) as st:
             size = query("ctr_diffattn_fwd_ws_size", C.byref(a))
@@ -247,19 +247,21 @@ def diff_attention_bwd(dout, q, k, v, lam, out, saved, causal=False, scale=None,
     shape = (a.B, a.T, a.H, 2 * a.D)
     if saved is None:
         raise ValueError("diff_attention_bwd: the forward ran with save=False")
-    o2, stat = saved
-    for t, what in ((dout, "dout"), (out, "out"), (o2, "saved")):
+    parts, stat = saved
+    for t, what in ((dout, "dout"), (out, "out")):
         if tuple(t.shape) != shape or t.dtype != q.dtype:
             raise ValueError(f"diff_attention_bwd: {what} of shape {shape} {q.dtype}, got {tuple(t.shape)} {t.dtype}")
-    if tuple(stat.shape) != (2, a.B * a.H * a.T) or stat.dtype != torch.float32:
+    if tuple(parts.shape) != (2, *shape) or parts.dtype != q.dtype or not parts.is_contiguous() or \
+            tuple(stat.shape) != (2, a.B * a.H * a.T) or stat.dtype != torch.float32 or not stat.is_contiguous():
         raise ValueError("diff_attention_bwd: saved as diff_attention_fwd gave it")
-    _device("diff_attention_bwd", q, dout, out, o2, stat)
-    dout, out, o2 = _aligned(dout), out.contiguous(), o2.contiguous()
+    _device("diff_attention_bwd", q, dout, out, parts, stat)
+    dout, out = _aligned(dout), _aligned(out.contiguous())
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
     dv = torch.empty(v.shape, dtype=q.dtype, device=q.device)
     dlam = torch.empty(a.H, dtype=torch.float32, device=q.device)
-    a.o, a.o2, a.stat = out.data_ptr(), o2.data_ptr(), stat.data_ptr()
+    a.o, a.stat = out.data_ptr(), stat.data_ptr()
+    a.o2, a.ol = parts.data_ptr(), parts.data_ptr() + 2 * out.numel()
     with _On(q) as st:
         size = query("ctr_diffattn_bwd_ws_size", C.byref(a))
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
