@@ -719,6 +719,19 @@ typedef struct {
 size_t ctr_newton_schulz_ws_size(const ctr_ns_mat_t* mats, int count);
 int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps, float a, float b, float c, float eps, int type,
                       void* ws, size_t ws_bytes, void* stream);
+/* The Muon update around it, fp32, a list of matrices of n elements.  apply = 0: buf = mu buf + g', u = g' + mu buf (nesterov)
+ * or buf, with g' = *coef g (coef on the device: the clip's multiplier).  Then ctr_newton_schulz on u, in place.  apply = 1:
+ * p = (1 - lr weight_decay) p - lr scale u.                                                              */
+typedef struct {
+  float *p, *buf;
+  const float* g;
+  float* u;
+  long n;
+  float scale;
+  int pad;
+} ctr_muon_mat_t;
+int ctr_muon_update(const ctr_muon_mat_t* mats, int count, int apply, const float* coef, float mu, int nesterov, float lr,
+                    float weight_decay, void* stream);
 
 #ifdef __cplusplus
 }

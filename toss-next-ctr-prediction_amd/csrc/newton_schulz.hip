@@ -581,6 +581,31 @@ __global__ __launch_bounds__(512, 2) void ns_small(const NsSmallArgs p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------ the update around it
+constexpr int MUON_MAXMAT = 64;
+struct MuonArgs {
+  const float* coef;       // the clip's multiplier of the gradients, on the device
+  float mu, lr, decay;
+  int nesterov;
+  ctr_muon_mat_t mat[MUON_MAXMAT];
+};
+// buf = mu buf + coef g;  u = coef g + mu buf (Nesterov) or buf
+__global__ __launch_bounds__(256) void muon_momentum(const MuonArgs a) {
+  const ctr_muon_mat_t& q = a.mat[blockIdx.y];
+  const float c = *a.coef;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < q.n; i += (long)gridDim.x * 256) {
+    const float g = c * q.g[i], b = fmaf(a.mu, q.buf[i], g);
+    q.buf[i] = b;
+    q.u[i] = a.nesterov ? fmaf(a.mu, b, g) : b;
+  }
+}
+// p = (1 - lr decay) p - lr scale u
+__global__ __launch_bounds__(256) void muon_apply(const MuonArgs a) {
+  const ctr_muon_mat_t& q = a.mat[blockIdx.y];
+  const float keep = 1.f - a.lr * a.decay, f = -a.lr * q.scale;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < q.n; i += (long)gridDim.x * 256) q.p[i] = fmaf(f, q.u[i], keep * q.p[i]);
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 // Layout of a matrix of the large form in the workspace; returns the bytes used.
 size_t ns_layout(NsMat& q, size_t off) {
@@ -782,4 +807,24 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
   flush_large(0);
   flush_large(1);
   return check_launch("newton_schulz");
+}
+
+extern "C" int ctr_muon_update(const ctr_muon_mat_t* mats, int count, int apply, const float* coef, float mu, int nesterov, float lr,
+                               float weight_decay, void* stream) {
+  CTR_REQUIRE(count >= 0 && (count == 0 || mats), "matrix list");
+  CTR_REQUIRE(apply || coef, "null coefficient");
+  MuonArgs a = {coef, mu, lr, weight_decay, nesterov, {}};
+  for (int i = 0; i < count; i += MUON_MAXMAT) {
+    const int n = std::min(MUON_MAXMAT, count - i);
+    long most = 0;
+    for (int k = 0; k < n; ++k) {
+      a.mat[k] = mats[i + k];
+      CTR_REQUIRE(a.mat[k].n >= 0 && a.mat[k].u && (apply ? (bool)a.mat[k].p : a.mat[k].g && a.mat[k].buf), "null matrix");
+      most = std::max(most, a.mat[k].n);
+    }
+    const dim3 grid(std::max(1, std::min(256, cdiv(most, 1024))), n);
+    if (apply) muon_apply<<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    else muon_momentum<<<grid, 256, 0, (hipStream_t)stream>>>(a);
+  }
+  return check_launch("muon_update");
 }

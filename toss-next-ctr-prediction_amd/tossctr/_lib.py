@@ -61,6 +61,10 @@ class NsMat(C.Structure):
     _fields_ = [("src", p), ("dst", p), ("ld_src", l), ("ld_dst", l), ("rows", i), ("cols", i)]
 
 
+class MuonMat(C.Structure):
+    _fields_ = [("p", p), ("buf", p), ("g", p), ("u", p), ("n", l), ("scale", f), ("pad", i)]
+
+
 class LazyTab(C.Structure):
     _fields_ = [("p_off", C.c_int64), ("rows", C.c_int64), ("width", C.c_int32), ("key_base", C.c_uint32),
                 ("last", p)]
@@ -216,6 +220,7 @@ SIGS = {
     "ctr_diffattn_bwd": (i, [C.POINTER(DiffAttn), p, l, l, l, p, p, p, p, p, z, p]),
     "ctr_newton_schulz_ws_size": (z, [C.POINTER(NsMat), i]),
     "ctr_newton_schulz": (i, [C.POINTER(NsMat), i, i, f, f, f, f, i, p, z, p]),
+    "ctr_muon_update": (i, [C.POINTER(MuonMat), i, i, p, f, i, f, f, p]),
 }
 
 _lib = None

@@ -219,8 +219,7 @@ class FusedAdamW:
         """Segment table: dense-grad region, no-grad region, then one sparse segment per table."""
         ar, eng, a = self.arena, self.engine, self.engine.a
         segs = []
-        if ar.n_dense_grad > 0:
-            segs.append(dict(p_off=0, n=ar.n_dense_grad, width=1, kind=0, g_off=0))
+        segs += self._dense_segments()
         lo, hi = ar.nograd_range
         if hi > lo:
             segs.append(dict(p_off=lo, n=hi - lo, width=1, kind=2, g_off=0))
@@ -238,6 +237,14 @@ class FusedAdamW:
                              n_uniq=ptr(t["n_uniq"]) if t else None, g_ld=t["G"].shape[1] if t else 0,
                              key_base=base, name=name))
         return segs
+
+    def _dense_segments(self):
+        """The dense params with grads: one AdamW segment."""
+        n = self.arena.n_dense_grad
+        return [dict(p_off=0, n=n, width=1, kind=0, g_off=0)] if n > 0 else []
+
+    def _step_matrices(self, g, st):
+        """Parameters that another rule updates, between the clip and the AdamW / EMA launches (FusedMuon)."""
 
     def _build_chunks(self):
         segs = self._segments(None)
@@ -496,6 +503,7 @@ class FusedAdamW:
         self.clip(tg, rows)
         self.step_count += 1
         st = self.engine.s()
+        self._step_matrices(g, st)
         if self._timing:
             ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
             ev[0].record()
@@ -534,3 +542,81 @@ class FusedAdamW:
 
     def zero_grad(self, set_to_none=True):
         pass   # grads are overwritten every backward
+
+
+def muon_keys(arch_order, shapes, kind, n_dense_grad, offsets):
+    """The parameters that Muon takes: the 2-D dense weights that map features to features.  Tables, per-feature embeddings and
+    position biases (rows are looked up, not multiplied), single-output heads and vectors stay with AdamW."""
+    return [k for k in arch_order
+            if kind[k] == "dense" and offsets[k] < n_dense_grad and len(shapes[k]) == 2 and min(shapes[k]) >= 2
+            and k not in ("num_embed.weight", "mask_embed.weight") and not k.endswith("pbias.rel.weight")]
+
+
+class FusedMuon(FusedAdamW):
+    """FusedAdamW whose dense weight matrices take the Muon rule instead: momentum of the clipped gradients (Nesterov), its
+    direction orthogonalised by Newton-Schulz (csrc/newton_schulz.hip), decoupled weight decay,
+        p <- (1 - lr wd) p - lr 0.2 sqrt(max(rows, cols)) O.
+    The factor gives O the root mean square of an AdamW step, so the learning rate and its schedule are AdamW's.  The momentum
+    is the matrices' part of ``m``; everything else (tables, vectors, clip, EMA, data parallel) is FusedAdamW's."""
+
+    def __init__(self, model, lr, weight_decay=1e-2, betas=(0.9, 0.999), eps=1e-8, max_grad_norm=0.0, ema=None,
+                 process_group=None, lazy=True, momentum=0.95, nesterov=True, ns_steps=5):
+        if not 0 <= momentum < 1:
+            raise ValueError(f"momentum in [0, 1), got {momentum}")
+        if not 1 <= int(ns_steps) <= 64:
+            raise ValueError(f"ns_steps in [1, 64], got {ns_steps}")
+        self.momentum, self.nesterov, self.ns_steps = float(momentum), bool(nesterov), int(ns_steps)
+        ar = model.arena
+        self.muon_params = muon_keys(ar.order, ar.shapes, ar.kind, ar.n_dense_grad, ar.offsets)
+        super().__init__(model, lr, weight_decay, betas, eps, max_grad_norm, ema, process_group, lazy)
+        self._build_muon()
+
+    def _dense_segments(self):
+        """AdamW runs between the matrices (a parameter starts on a 64-element boundary), the matrices as EMA-only segments."""
+        ar, segs, at = self.arena, [], 0
+        for k in sorted(self.muon_params, key=ar.offsets.get):
+            o, n = ar.offsets[k], int(np.prod(ar.shapes[k]))
+            if o > at:
+                segs.append(dict(p_off=at, n=o - at, width=1, kind=0, g_off=at))
+            segs.append(dict(p_off=o, n=n, width=1, kind=2, g_off=0))
+            at = (o + n + 63) // 64 * 64
+        if ar.n_dense_grad > at:
+            segs.append(dict(p_off=at, n=ar.n_dense_grad - at, width=1, kind=0, g_off=at))
+        return segs
+
+    def _build_muon(self):
+        ar, keys = self.arena, self.muon_params
+        sizes = [int(np.prod(ar.shapes[k])) for k in keys]
+        self._muon_u = torch.empty(max(1, sum((n + 63) // 64 * 64 for n in sizes)), dtype=torch.float32, device=ar.device)
+        self._muon_mats = (_lib.MuonMat * max(1, len(keys)))()
+        self._ns_mats = (_lib.NsMat * max(1, len(keys)))()
+        at = 0
+        for e, s, k, n in zip(self._muon_mats, self._ns_mats, keys, sizes):
+            o, (rows, cols) = ar.offsets[k], ar.shapes[k]
+            e.p, e.buf, e.g, e.u = ptr(ar.buf, o), ptr(self.m, o), ptr(ar.grad, o), ptr(self._muon_u, at)
+            e.n, e.scale = n, 0.2 * math.sqrt(max(rows, cols))
+            s.src = s.dst = ptr(self._muon_u, at)
+            s.ld_src = s.ld_dst = s.cols = cols
+            s.rows = rows
+            at += (n + 63) // 64 * 64
+        size = _lib.query("ctr_newton_schulz_ws_size", self._ns_mats, len(keys))
+        self._ns_ws = torch.empty(max(1, size), dtype=torch.uint8, device=ar.device)
+
+    def _step_matrices(self, g, st):
+        n = len(self.muon_params)
+        if n == 0:
+            return
+        from .ops import NS_COEFFS
+        lr, wd = float(g["lr"]), float(g["weight_decay"])
+        call("ctr_muon_update", self._muon_mats, n, 0, ptr(self.norm_out, 1), self.momentum, int(self.nesterov), lr, wd, st)
+        call("ctr_newton_schulz", self._ns_mats, n, self.ns_steps, *NS_COEFFS, 1e-7, 0, ptr(self._ns_ws),
+             self._ns_ws.numel(), st)
+        call("ctr_muon_update", self._muon_mats, n, 1, None, self.momentum, int(self.nesterov), lr, wd, st)
+
+
+def build_optimizer(model, cfg, ema=None, process_group=None):
+    """The optimizer that ``train.optimizer`` names: "muon" is FusedMuon, anything else the reference's AdamW."""
+    tr = cfg["train"]
+    cls = FusedMuon if str(tr.get("optimizer", "adamw")).lower() == "muon" else FusedAdamW
+    return cls(model, lr=tr["lr"], weight_decay=tr["weight_decay"], max_grad_norm=tr.get("grad_clip_norm", 0.0), ema=ema,
+               process_group=process_group)

@@ -180,7 +180,7 @@ def train_one_fold(cfg, fold, idx_tr, idx_va, manifest_path, logger, store=None,
     from .configs import cat_cardinals  # noqa: F401
     from .data import DeviceShards
     from .metrics import Calibrator, DeviceMetrics, final_score
-    from .optim import FusedAdamW, build_ema
+    from .optim import build_ema, build_optimizer
     from .wrapper import CTRModel
     dist = _dist()
     world = dist.get_world_size() if dist else 1
@@ -199,9 +199,7 @@ def train_one_fold(cfg, fold, idx_tr, idx_va, manifest_path, logger, store=None,
                      process_group=dist.group.WORLD if dist else None, shard_tables=shard)
     model.reset_parameters(torch.Generator(device=device).manual_seed(int(cfg.get("seed", 777)) + fold))
     ema = build_ema(model, cfg)
-    opt = FusedAdamW(model, lr=cfg["train"]["lr"], weight_decay=cfg["train"]["weight_decay"],
-                     max_grad_norm=cfg["train"].get("grad_clip_norm", 0.0), ema=ema,
-                     process_group=dist.group.WORLD if dist else None)
+    opt = build_optimizer(model, cfg, ema=ema, process_group=dist.group.WORLD if dist else None)
     y_host = store.t["y"].view(-1).cpu().numpy()
     idx_tr = np.asarray(idx_tr, dtype=np.int64)
     steps_per_epoch = math.ceil(len(idx_tr) / (bs * world))
