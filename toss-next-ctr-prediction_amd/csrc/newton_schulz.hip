@@ -174,22 +174,24 @@ __device__ __forceinline__ void ns_wait() {      // all but the last N loads hav
 }
 
 // A tile of 64 WR x 128 of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.
-// 2 WR waves of 64 x 64.  A K step's four planes come by direct loads to one of NST places in LDS, NST - 1 steps ahead:
-// eight waves (WR = 4) and three places where there are tiles for every compute unit -- the step's products last shorter
-// than a load, so one step ahead is not enough, and the larger tile reads a quarter less --, four waves and four places
-// where a tile's chain of steps is what counts.  Rows of 64 bytes (k) hold their 16-byte chunk c at c ^ (row / 4 % 4), rows
+// WR CW = 8 waves of 64 x 128 / CW, two a SIMD: one's products run under the other's LDS reads (four waves of 64 x 64 took
+// 0.86 us a step, the sum of both).  A K step's four planes come by direct loads to one of NST places in LDS, NST - 1 steps
+// ahead -- a step's products last shorter than a load, so one is not enough: 256 x 128 (WR = 4) and three places for large
+// matrices, where the larger tile reads a quarter less, 128 x 128 and four places where a tile's chain of steps is what
+// counts.  Rows of 64 bytes (k) hold their 16-byte chunk c at c ^ (row / 4 % 4), rows
 // of 256 bytes (columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads then cover all banks.
 template <int WR> constexpr int ns_stage() { return 2 * NS_BK * (64 * WR + NS_TILE); }      // elements of a step's planes
-template <bool NN, int WR, int NST>
+template <bool NN, int WR, int CW, int NST>
 __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda, const _Float16* B, long planeB, int ldb,
-                                        int r0, int c0, int k0, int k1, _Float16* lds, f32x16 acc[2][2]) {
-  constexpr int PA = 64 * WR * NS_BK, PB = NS_TILE * NS_BK, STAGE = ns_stage<WR>(), NB = 8 / WR, LOADS = 4 + NB;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+                                        int r0, int c0, int k0, int k1, _Float16* lds, f32x16 (&acc)[2][4 / CW]) {
+  constexpr int PA = 64 * WR * NS_BK, PB = NS_TILE * NS_BK, STAGE = ns_stage<WR>(), NJ = 4 / CW;
+  constexpr int SHARE = WR * CW / 2, NA = 4 * WR / SHARE, NB = 8 / SHARE, LOADS = NA + NB;      // waves of a plane, a wave's loads of it
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / CW * 64, wc = wave % CW * (NS_TILE / CW);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
-  // wave w loads of plane w / WR the A rows 64 (w % WR) .., and that share of the B rows or K rows
-  const int pl = wave / WR, sh = wave % WR;
-  const _Float16* asrc = A + pl * planeA + (long)(r0 + 64 * sh) * lda + k0;
-  const _Float16* bsrc = B + pl * planeB + (NN ? (long)(k0 + NS_BK / WR * sh) * ldb + c0 : (long)(c0 + NS_TILE / WR * sh) * ldb + k0);
+  // wave w loads of plane w / SHARE its share of the A rows and of the B rows or K rows
+  const int pl = wave / SHARE, sh = wave % SHARE;
+  const _Float16* asrc = A + pl * planeA + (long)(r0 + 16 * NA * sh) * lda + k0;
+  const _Float16* bsrc = B + pl * planeB + (NN ? (long)(k0 + 4 * NB * sh) * ldb + c0 : (long)(c0 + 16 * NB * sh) * ldb + k0);
   const uint32_t aoff = (lane >> 2) * lda * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
   uint32_t boff[NB];
 #pragma unroll
@@ -199,16 +201,16 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda,
   const auto stage = [&](int step, int place) {
     const auto ra = buf_rsrc(asrc + (long)step * NS_BK, 0x7ffffff0u);
     const auto rb = buf_rsrc(bsrc + (long)step * NS_BK * (NN ? ldb : 1), 0x7ffffff0u);
-    const uint32_t ta = lds0 + (place * STAGE + pl * PA + sh * 64 * NS_BK) * 2, tb = lds0 + (place * STAGE + 2 * PA + pl * PB + sh * (PB / WR)) * 2;
+    const uint32_t ta = lds0 + (place * STAGE + pl * PA + sh * (PA / SHARE)) * 2, tb = lds0 + (place * STAGE + 2 * PA + pl * PB + sh * (PB / SHARE)) * 2;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ns_dma16(ra, ta + j * 1024, aoff, j * 32 * lda);
+    for (int j = 0; j < NA; ++j) ns_dma16(ra, ta + j * 1024, aoff, j * 32 * lda);
 #pragma unroll
     for (int j = 0; j < NB; ++j) ns_dma16(rb, tb + j * 1024, boff[j], j * (NN ? 8 : 32) * ldb);
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < NJ; ++j) acc[i][j] = 0.f;
   const int steps = (k1 - k0) / NS_BK;
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i)
@@ -216,42 +218,59 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda,
   const int row = lane & 31, h = lane >> 5;
   const int arow = (wr + row) * NS_BK, brow = (wc + row) * NS_BK, turn = (row >> 2) & 3;
   const int tk = 8 * h + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;      // transpose reads: row, column
+  struct Frags { f16x8 a[2][2], b[2][NJ]; };      // [plane][tile]
+  const auto read = [&](int place, int kk) {
+    const _Float16* s = lds + place * STAGE;
+    const int ch = ((2 * kk + h) ^ turn) * 8;
+    Frags f;
+#pragma unroll
+    for (int pl = 0; pl < 2; ++pl) {
+      const _Float16* bp = s + 2 * PA + pl * PB;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f.a[pl][i] = *(const f16x8*)(s + pl * PA + arow + 32 * i * NS_BK + ch);
+#pragma unroll
+      for (int i = 0; i < NJ; ++i) {
+        if constexpr (!NN) f.b[pl][i] = *(const f16x8*)(bp + brow + 32 * i * NS_BK + ch);
+        else {
+          f16x4 u[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int r = 16 * kk + tk + 4 * half, c = wc + 32 * i + tc;
+            const _Float16* q = bp + r * NS_TILE + ((c >> 3) ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (c & 4);
+            u[half] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
+          }
+          f.b[pl][i] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      }
+    }
+    return f;
+  };
+  const auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int pr = 0; pr < 3; ++pr)      // lo hi, hi lo, hi hi; the accumulators in turn
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = MFMA16(f.a[pr == 0][i], f.b[pr == 1][j], acc[i][j]);
+  };
+  // Half a step's fragments are read while the half before is multiplied; the barrier, in the middle of a step, is where the
+  // next one has landed and the place of the last one is free.
+  if (steps <= 0) return;
+  if (steps >= NST - 1) ns_wait<LOADS * (NST - 2)>();
+  else ns_wait<0>();
+  Frags f = read(0, 0);
   int place = 0;
   for (int k = 0; k < steps; ++k) {
-    if (k + NST - 1 <= steps) ns_wait<LOADS * (NST - 2)>();
-    else ns_wait<0>();
-    if (k + NST - 1 < steps) stage(k + NST - 1, place == 0 ? NST - 1 : place - 1);
-    const _Float16* s = lds + place * STAGE;
-    place = place + 1 == NST ? 0 : place + 1;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      f16x8 a[2][2], b[2][2];      // [plane][tile]
-      const int ch = ((2 * kk + h) ^ turn) * 8;
-#pragma unroll
-      for (int pl = 0; pl < 2; ++pl)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          a[pl][i] = *(const f16x8*)(s + pl * PA + arow + 32 * i * NS_BK + ch);
-          const _Float16* bp = s + 2 * PA + pl * PB;
-          if constexpr (!NN) b[pl][i] = *(const f16x8*)(bp + brow + 32 * i * NS_BK + ch);
-          else {
-            f16x4 u[2];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int r = 16 * kk + tk + 4 * half, c = wc + 32 * i + tc;
-              const _Float16* q = bp + r * NS_TILE + ((c >> 3) ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (c & 4);
-              u[half] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
-            }
-            b[pl][i] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7);
-          }
-        }
-#pragma unroll
-      for (int pr = 0; pr < 3; ++pr)      // lo hi, hi lo, hi hi; four accumulators in turn
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i][j] = MFMA16(a[pr == 0][i], b[pr == 1][j], acc[i][j]);
+    const Frags g = read(place, 1);
+    multiply(f);
+    if (k + 1 < steps) {
+      if (k + NST - 1 <= steps) ns_wait<LOADS * (NST - 3)>();
+      else ns_wait<0>();
+      if (k + NST - 1 < steps) stage(k + NST - 1, place == 0 ? NST - 1 : place - 1);
+      place = place + 1 == NST ? 0 : place + 1;
+      f = read(place, 0);
     }
+    multiply(g);
   }
 }
 
@@ -279,8 +298,8 @@ __host__ __device__ inline int tri_tiles(int mp, int wr) {
 
 // partials of X X^T (square = false) or A A over a share of K, lower tiles; the workgroups of an XCD (every eighth) take the
 // same share, whose rows so stay in its L2
-template <int WR, int NST>
-__global__ __launch_bounds__(128 * WR, 1) void ns_gram(const NsArgs p, int buf, bool square) {
+template <int WR, int CW, int NST>
+__global__ __launch_bounds__(64 * WR * CW, 1) void ns_gram(const NsArgs p, int buf, bool square) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
@@ -292,19 +311,20 @@ __global__ __launch_bounds__(128 * WR, 1) void ns_gram(const NsArgs p, int buf, 
   const int steps = K / NS_BK, per = (steps + splits - 1) / splits;
   const long plane = (long)q.mp * K;
   const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
-  f32x16 acc[2][2];
-  ns_tile<false, WR, NST>(x, plane, K, x, plane, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
+  constexpr int NJ = 4 / CW;
+  f32x16 acc[2][NJ];
+  ns_tile<false, WR, CW, NST>(x, plane, K, x, plane, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
                       min(steps, (sp + 1) * per) * NS_BK, lds, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < NJ; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        out[(long)(ti * 64 * WR + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * NS_TILE + (wave & 1) * 64 +
-            b * 32 + (lane & 31)] = acc[a][b][r];
+        out[(long)(ti * 64 * WR + wave / CW * 64 + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * NS_TILE +
+            wave % CW * (NS_TILE / CW) + b * 32 + (lane & 31)] = acc[a][b][r];
 }
 
 // the partials of a 32 x 32 block of the lower tiles summed in order (four elements a thread, eight loads in flight), and A
@@ -365,8 +385,8 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
 
 // X' = W X; the last step writes the result in its own type and orientation.  An XCD takes every eighth panel of columns, with
 // all row tiles of one together.
-template <int WR, int NST>
-__global__ __launch_bounds__(128 * WR, 1) void ns_apply(const NsArgs p, int buf, int last) {
+template <int WR, int CW, int NST>
+__global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int buf, int last) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
@@ -376,19 +396,20 @@ __global__ __launch_bounds__(128 * WR, 1) void ns_apply(const NsArgs p, int buf,
   const _Float16* W = (const _Float16*)(p.ws + q.off_a) + 2 * planeW;
   const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
   _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
-  f32x16 acc[2][2];
-  ns_tile<true, WR, NST>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
+  constexpr int NJ = 4 / CW;
+  f32x16 acc[2][NJ];
+  ns_tile<true, WR, CW, NST>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool tall = q.rows > q.cols;
   if (last) {
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int c = c0 + (wave & 1) * 64 + b * 32 + (lane & 31);
+      for (int b = 0; b < NJ; ++b) {
+        const int c = c0 + wave % CW * (NS_TILE / CW) + b * 32 + (lane & 31);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int row = r0 + (wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5);
+          const int row = r0 + wave / CW * 64 + a * 32 + c_row(r, lane >> 5);
           if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, acc[a][b][r] * (1.f / (SA * SX)));
         }
       }
@@ -400,17 +421,17 @@ __global__ __launch_bounds__(128 * WR, 1) void ns_apply(const NsArgs p, int buf,
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < NJ; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int o = ((wave >> 1) * 64 + a * 32 + c_row(r, lane >> 5)) * LD + (wave & 1) * 64 + b * 32 + (lane & 31);
+        const int o = (wave / CW * 64 + a * 32 + c_row(r, lane >> 5)) * LD + wave % CW * (NS_TILE / CW) + b * 32 + (lane & 31);
         split16(acc[a][b][r] * (1.f / SA), lds[o], lds[PL + o]);
       }
   __syncthreads();
-  constexpr int PER = 2 * 64 * WR * (NS_TILE / 8) / (128 * WR);
+  constexpr int PER = 2 * 64 * WR * (NS_TILE / 8) / (64 * WR * CW);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int e = threadIdx.x + k * 128 * WR, c = e % (NS_TILE / 8), row = e / (NS_TILE / 8) % (64 * WR), pl = e / (NS_TILE / 8) / (64 * WR);
+    const int e = threadIdx.x + k * 64 * WR * CW, c = e % (NS_TILE / 8), row = e / (NS_TILE / 8) % (64 * WR), pl = e / (NS_TILE / 8) / (64 * WR);
     *(f16x8*)(y + pl * plane + (long)(r0 + row) * q.np + c0 + c * 8) = *(const f16x8*)(lds + pl * PL + row * LD + c * 8);
   }
 }
@@ -687,8 +708,8 @@ bool ns_allow_lds() {
   const auto allow = [](const void* f, int n) {
     return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n) == hipSuccess;
   };
-  if (!allow((const void*)ns_gram<4, 3>, NS_LDS4) || !allow((const void*)ns_gram<2, 4>, NS_LDS2) ||
-      !allow((const void*)ns_apply<4, 3>, NS_LDS4) || !allow((const void*)ns_apply<2, 4>, NS_LDS2) ||
+  if (!allow((const void*)ns_gram<4, 2, 3>, NS_LDS4) || !allow((const void*)ns_gram<2, 4, 4>, NS_LDS2) ||
+      !allow((const void*)ns_apply<4, 2, 3>, NS_LDS4) || !allow((const void*)ns_apply<2, 4, 4>, NS_LDS2) ||
       !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
       !allow((const void*)ns_small<__bf16>, NS_SMALL_LDS) || !allow((const void*)ns_small<_Float16>, NS_SMALL_LDS))
     return false;
@@ -776,14 +797,14 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     for (int k = 0; k < steps; ++k) {
       for (int square = 0; square < 2; ++square) {
         const int ng = prefix([&](const NsMat& q) { return cdiv(square ? q.asplits : q.splits, 8) * 8 * tri_tiles(q.mp, q.wr); });
-        if (w) ns_gram<4, 3><<<ng, 512, NS_LDS4, s>>>(g, k & 1, square);
-        else ns_gram<2, 4><<<ng, 256, NS_LDS2, s>>>(g, k & 1, square);
+        if (w) ns_gram<4, 2, 3><<<ng, 512, NS_LDS4, s>>>(g, k & 1, square);
+        else ns_gram<2, 4, 4><<<ng, 512, NS_LDS2, s>>>(g, k & 1, square);
         const int nj = prefix([](const NsMat& q) { return (q.mp / 32) * (q.mp / 32 + 1) / 2; });
         ns_join<<<nj, 256, 0, s>>>(g, square);
       }
       const int na = prefix([](const NsMat& q) { return q.mp / (64 * q.wr) * (cdiv(q.np / NS_TILE, 8) * 8); });
-      if (w) ns_apply<4, 3><<<na, 512, NS_LDS4, s>>>(g, k & 1, k + 1 == steps);
-      else ns_apply<2, 4><<<na, 256, NS_LDS2, s>>>(g, k & 1, k + 1 == steps);
+      if (w) ns_apply<4, 2, 3><<<na, 512, NS_LDS4, s>>>(g, k & 1, k + 1 == steps);
+      else ns_apply<2, 4, 4><<<na, 512, NS_LDS2, s>>>(g, k & 1, k + 1 == steps);
     }
     g.count = 0;
     off[w] = 0;
