@@ -61,6 +61,10 @@ __device__ __forceinline__ void ns_store(const NsMat& q, int r, int c, float v) 
   else ((_Float16*)q.dst)[o] = (_Float16)v;
 }
 
+// The planes in the workspace: 32 hi, then the same 32 lo values, so that a K step of a row is one line of 128 bytes (with a
+// plane after the other it was half a line of each, and twice the requests).  Where hi of (row, col) stands; lo: 32 further.
+__device__ __forceinline__ long at(long row, int col, int ld) { return row * 2 * ld + (col >> 5) * 64 + (col & 31); }
+
 __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
@@ -152,11 +156,10 @@ __global__ __launch_bounds__(256) void ns_init(const NsArgs p) {
   }
   __syncthreads();
   _Float16* x = (_Float16*)(p.ws + q.off_x);
-  const long plane = (long)q.mp * q.np;
   for (int j = ly; j < 64; j += 4) {
     const float v = tall ? tile[lx][j] : tile[j][lx];
-    const long o = (long)(m0 + j) * q.np + n0 + lx;
-    split16(v * scale, x[o], x[plane + o]);
+    const long o = at(m0 + j, n0 + lx, q.np);
+    split16(v * scale, x[o], x[o + 32]);
   }
 }
 
@@ -178,34 +181,34 @@ __device__ __forceinline__ void ns_wait() {      // all but the last N loads hav
 // 0.86 us a step, the sum of both).  A K step's four planes come by direct loads to one of NST places in LDS, NST - 1 steps
 // ahead -- a step's products last shorter than a load, so one is not enough: 256 x 128 (WR = 4) and three places for large
 // matrices, where the larger tile reads a quarter less, 128 x 128 and four places where a tile's chain of steps is what
-// counts.  Rows of 64 bytes (k) hold their 16-byte chunk c at c ^ (row / 4 % 4), rows
-// of 256 bytes (columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads then cover all banks.
+// counts.  In LDS a row of 128 bytes (A, NT: hi and lo of 32 k) holds its 16-byte chunk c at c ^ (row / 2 % 8), one of 512
+// bytes (NN: hi and lo of 128 columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads cover all banks.
 template <int WR> constexpr int ns_stage() { return 2 * NS_BK * (64 * WR + NS_TILE); }      // elements of a step's planes
 template <bool NN, int WR, int CW, int NST>
-__device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda, const _Float16* B, long planeB, int ldb,
-                                        int r0, int c0, int k0, int k1, _Float16* lds, f32x16 (&acc)[2][4 / CW]) {
-  constexpr int PA = 64 * WR * NS_BK, PB = NS_TILE * NS_BK, STAGE = ns_stage<WR>(), NJ = 4 / CW;
-  constexpr int SHARE = WR * CW / 2, NA = 4 * WR / SHARE, NB = 8 / SHARE, LOADS = NA + NB;      // waves of a plane, a wave's loads of it
+__device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float16* B, int ldb, int r0, int c0, int k0, int k1,
+                                        _Float16* lds, f32x16 (&acc)[2][4 / CW]) {
+  static_assert(WR * CW == 8, "eight waves deal out the loads");
+  constexpr int PA = 2 * 64 * WR * NS_BK, STAGE = ns_stage<WR>(), NJ = 4 / CW, LOADS = WR + 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / CW * 64, wc = wave % CW * (NS_TILE / CW);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
-  // wave w loads of plane w / SHARE its share of the A rows and of the B rows or K rows
-  const int pl = wave / SHARE, sh = wave % SHARE;
-  const _Float16* asrc = A + pl * planeA + (long)(r0 + 16 * NA * sh) * lda + k0;
-  const _Float16* bsrc = B + pl * planeB + (NN ? (long)(k0 + 4 * NB * sh) * ldb + c0 : (long)(c0 + 16 * NB * sh) * ldb + k0);
-  const uint32_t aoff = (lane >> 2) * lda * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
-  uint32_t boff[NB];
+  // a load is 8 rows of 128 bytes, or 2 of 512; wave w takes WR of A and two of B
+  const _Float16* asrc = A + at(r0 + 8 * WR * wave, k0, lda);
+  const _Float16* bsrc = B + (NN ? at(k0 + 4 * wave, c0, ldb) : at(c0 + 16 * wave, k0, ldb));
+  uint32_t aoff[2], boff[2];
 #pragma unroll
-  for (int j = 0; j < NB; ++j)
-    boff[j] = NN ? (lane >> 4) * ldb * 2 + (((lane & 15) ^ ((lane >> 4) << 2)) ^ ((NB * sh + j) & 3)) * 16
-                 : (lane >> 2) * ldb * 2 + ((lane & 3) ^ (lane >> 4)) * 16;
+  for (int j = 0; j < 2; ++j) {
+    aoff[j] = (lane >> 3) * lda * 4 + ((lane & 7) ^ ((4 * (WR * wave + j) + (lane >> 4)) & 7)) * 16;
+    boff[j] = NN ? (lane >> 5) * ldb * 4 + ((lane & 31) ^ ((((2 * j + (lane >> 5)) & 3) << 2) | (wave & 3))) * 16
+                 : (lane >> 3) * ldb * 4 + ((lane & 7) ^ ((4 * j + (lane >> 4)) & 7)) * 16;
+  }
   const auto stage = [&](int step, int place) {
-    const auto ra = buf_rsrc(asrc + (long)step * NS_BK, 0x7ffffff0u);
-    const auto rb = buf_rsrc(bsrc + (long)step * NS_BK * (NN ? ldb : 1), 0x7ffffff0u);
-    const uint32_t ta = lds0 + (place * STAGE + pl * PA + sh * (PA / SHARE)) * 2, tb = lds0 + (place * STAGE + 2 * PA + pl * PB + sh * (PB / SHARE)) * 2;
+    const auto ra = buf_rsrc(asrc + (long)step * 2 * NS_BK, 0x7ffffff0u);
+    const auto rb = buf_rsrc(bsrc + (NN ? (long)step * 2 * NS_BK * ldb : (long)step * 2 * NS_BK), 0x7ffffff0u);
+    const uint32_t ta = lds0 + (place * STAGE + wave * WR * 512) * 2, tb = lds0 + (place * STAGE + PA + wave * 1024) * 2;
 #pragma unroll
-    for (int j = 0; j < NA; ++j) ns_dma16(ra, ta + j * 1024, aoff, j * 32 * lda);
+    for (int j = 0; j < WR; ++j) ns_dma16(ra, ta + j * 1024, aoff[j & 1], j * 32 * lda);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) ns_dma16(rb, tb + j * 1024, boff[j], j * (NN ? 8 : 32) * ldb);
+    for (int j = 0; j < 2; ++j) ns_dma16(rb, tb + j * 1024, boff[j], j * (NN ? 8 : 32) * ldb);
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -215,28 +218,28 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, long planeA, int lda,
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i)
     if (i < steps) stage(i, i);
-  const int row = lane & 31, h = lane >> 5;
-  const int arow = (wr + row) * NS_BK, brow = (wc + row) * NS_BK, turn = (row >> 2) & 3;
+  const int row = lane & 31, h = lane >> 5, turn = (row >> 1) & 7;
+  const int arow = (wr + row) * 2 * NS_BK, brow = (wc + row) * 2 * NS_BK;
   const int tk = 8 * h + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;      // transpose reads: row, column
   struct Frags { f16x8 a[2][2], b[2][NJ]; };      // [plane][tile]
   const auto read = [&](int place, int kk) {
     const _Float16* s = lds + place * STAGE;
-    const int ch = ((2 * kk + h) ^ turn) * 8;
+    const _Float16* bp = s + PA;
     Frags f;
 #pragma unroll
     for (int pl = 0; pl < 2; ++pl) {
-      const _Float16* bp = s + 2 * PA + pl * PB;
+      const int ch = ((4 * pl + 2 * kk + h) ^ turn) * 8;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) f.a[pl][i] = *(const f16x8*)(s + pl * PA + arow + 32 * i * NS_BK + ch);
+      for (int i = 0; i < 2; ++i) f.a[pl][i] = *(const f16x8*)(s + arow + 64 * i * NS_BK + ch);
 #pragma unroll
       for (int i = 0; i < NJ; ++i) {
-        if constexpr (!NN) f.b[pl][i] = *(const f16x8*)(bp + brow + 32 * i * NS_BK + ch);
+        if constexpr (!NN) f.b[pl][i] = *(const f16x8*)(bp + brow + 64 * i * NS_BK + ch);
         else {
           f16x4 u[2];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int r = 16 * kk + tk + 4 * half, c = wc + 32 * i + tc;
-            const _Float16* q = bp + r * NS_TILE + ((c >> 3) ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (c & 4);
+            const int r = 16 * kk + tk + 4 * half, c = (wc / 32 + i) * 8 + 4 * pl + (tc >> 3);
+            const _Float16* q = bp + r * 2 * NS_TILE + (c ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (tc & 4);
             u[half] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
           }
           f.b[pl][i] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -309,11 +312,10 @@ __global__ __launch_bounds__(64 * WR * CW, 1) void ns_gram(const NsArgs p, int b
   int ti, tj;
   tri_tile<WR>((id >> 3) % tiles, ti, tj);
   const int steps = K / NS_BK, per = (steps + splits - 1) / splits;
-  const long plane = (long)q.mp * K;
-  const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
+  const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + (long)buf * 2 * q.mp * K;
   constexpr int NJ = 4 / CW;
   f32x16 acc[2][NJ];
-  ns_tile<false, WR, CW, NST>(x, plane, K, x, plane, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
+  ns_tile<false, WR, CW, NST>(x, K, x, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
                       min(steps, (sp + 1) * per) * NS_BK, lds, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -352,8 +354,8 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
   }
   for (; s < splits; ++s) v += *(const f32x4*)(in + s * plane);
   if (square) {
-    const long o = (long)(ti * 32 + r) * q.mp + tj * 32 + c4;
-    const f32x4 av = __builtin_convertvector(*(const f16x4*)(A + o), f32x4) + __builtin_convertvector(*(const f16x4*)(A + plane + o), f32x4);
+    const _Float16* o = A + at(ti * 32 + r, tj * 32 + c4, q.mp);
+    const f32x4 av = __builtin_convertvector(*(const f16x4*)o, f32x4) + __builtin_convertvector(*(const f16x4*)(o + 32), f32x4);
     v = p.b * av + (p.c / SA) * v;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -370,8 +372,8 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
       hi[k] = a;
       lo[k] = b;
     }
-    *(f16x4*)(out + (long)row * q.mp + col) = hi;
-    *(f16x4*)(out + plane + (long)row * q.mp + col) = lo;
+    *(f16x4*)(out + at(row, col, q.mp)) = hi;
+    *(f16x4*)(out + at(row, col, q.mp) + 32) = lo;
   };
   put(ti * 32 + r, tj * 32 + c4, v);
   if (ti == tj) return;      // the whole block: it is symmetric by itself
@@ -398,7 +400,7 @@ __global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int 
   _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
   constexpr int NJ = 4 / CW;
   f32x16 acc[2][NJ];
-  ns_tile<true, WR, CW, NST>(W, planeW, q.mp, x, plane, q.np, r0, c0, 0, q.mp, lds, acc);
+  ns_tile<true, WR, CW, NST>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool tall = q.rows > q.cols;
   if (last) {
@@ -432,7 +434,7 @@ __global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int 
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int e = threadIdx.x + k * 64 * WR * CW, c = e % (NS_TILE / 8), row = e / (NS_TILE / 8) % (64 * WR), pl = e / (NS_TILE / 8) / (64 * WR);
-    *(f16x8*)(y + pl * plane + (long)(r0 + row) * q.np + c0 + c * 8) = *(const f16x8*)(lds + pl * PL + row * LD + c * 8);
+    *(f16x8*)(y + at(r0 + row, c0 + c * 8, q.np) + pl * 32) = *(const f16x8*)(lds + pl * PL + row * LD + c * 8);
   }
 }
 
