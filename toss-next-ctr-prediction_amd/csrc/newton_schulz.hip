@@ -186,7 +186,7 @@ __device__ __forceinline__ void ns_wait() {      // all but the last N loads hav
 template <int WR> constexpr int ns_stage() { return 2 * NS_BK * (64 * WR + NS_TILE); }      // elements of a step's planes
 template <bool NN, int WR, int CW, int NST>
 __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float16* B, int ldb, int r0, int c0, int k0, int k1,
-                                        _Float16* lds, f32x16 (&acc)[2][4 / CW]) {
+                                        _Float16* lds, bool hi_only, f32x16 (&acc)[2][4 / CW]) {
   static_assert(WR * CW == 8, "eight waves deal out the loads");
   constexpr int PA = 2 * 64 * WR * NS_BK, STAGE = ns_stage<WR>(), NJ = 4 / CW, LOADS = WR + 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / CW * 64, wc = wave % CW * (NS_TILE / CW);
@@ -250,11 +250,13 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float
   };
   const auto multiply = [&](const Frags& f) {
 #pragma unroll
-    for (int pr = 0; pr < 3; ++pr)      // lo hi, hi lo, hi hi; the accumulators in turn
+    for (int pr = 0; pr < 3; ++pr) {    // lo hi, hi lo, hi hi; the accumulators in turn
+      if (pr < 2 && hi_only) continue;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = MFMA16(f.a[pr == 0][i], f.b[pr == 1][j], acc[i][j]);
+    }
   };
   // Half a step's fragments are read while the half before is multiplied; the barrier, in the middle of a step, is where the
   // next one has landed and the place of the last one is free.
@@ -302,7 +304,7 @@ __host__ __device__ inline int tri_tiles(int mp, int wr) {
 // partials of X X^T (square = false) or A A over a share of K, lower tiles; the workgroups of an XCD (every eighth) take the
 // same share, whose rows so stay in its L2
 template <int WR, int CW, int NST>
-__global__ __launch_bounds__(64 * WR * CW, 1) void ns_gram(const NsArgs p, int buf, bool square) {
+__global__ __launch_bounds__(64 * WR * CW, 1) void ns_gram(const NsArgs p, int buf, bool square, bool hi_only) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(64 * WR * CW, 1) void ns_gram(const NsArgs p, int b
   constexpr int NJ = 4 / CW;
   f32x16 acc[2][NJ];
   ns_tile<false, WR, CW, NST>(x, K, x, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
-                      min(steps, (sp + 1) * per) * NS_BK, lds, acc);
+                      min(steps, (sp + 1) * per) * NS_BK, lds, hi_only, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -388,7 +390,7 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
 // X' = W X; the last step writes the result in its own type and orientation.  An XCD takes every eighth panel of columns, with
 // all row tiles of one together.
 template <int WR, int CW, int NST>
-__global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int buf, int last) {
+__global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int buf, int last, bool hi_only) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int 
   _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
   constexpr int NJ = 4 / CW;
   f32x16 acc[2][NJ];
-  ns_tile<true, WR, CW, NST>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, acc);
+  ns_tile<true, WR, CW, NST>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, hi_only, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool tall = q.rows > q.cols;
   if (last) {
@@ -797,16 +799,19 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     const int ni = prefix([](const NsMat& q) { return q.mp / 64 * (q.np / 64); });
     ns_init<<<ni, 256, 0, s>>>(g);
     for (int k = 0; k < steps; ++k) {
+      // nothing multiplies the last step's error: a bf16 result (half a step 2^-8) takes its products from the hi parts alone,
+      // whose roundings, 2^-12 of each operand, add a twentieth to the result's own error
+      const bool hi_only = k + 1 == steps && steps > 1 && type == TY_BF16;
       for (int square = 0; square < 2; ++square) {
         const int ng = prefix([&](const NsMat& q) { return cdiv(square ? q.asplits : q.splits, 8) * 8 * tri_tiles(q.mp, q.wr); });
-        if (w) ns_gram<4, 2, 3><<<ng, 512, NS_LDS4, s>>>(g, k & 1, square);
-        else ns_gram<2, 4, 4><<<ng, 512, NS_LDS2, s>>>(g, k & 1, square);
+        if (w) ns_gram<4, 2, 3><<<ng, 512, NS_LDS4, s>>>(g, k & 1, square, hi_only);
+        else ns_gram<2, 4, 4><<<ng, 512, NS_LDS2, s>>>(g, k & 1, square, hi_only);
         const int nj = prefix([](const NsMat& q) { return (q.mp / 32) * (q.mp / 32 + 1) / 2; });
         ns_join<<<nj, 256, 0, s>>>(g, square);
       }
       const int na = prefix([](const NsMat& q) { return q.mp / (64 * q.wr) * (cdiv(q.np / NS_TILE, 8) * 8); });
-      if (w) ns_apply<4, 2, 3><<<na, 512, NS_LDS4, s>>>(g, k & 1, k + 1 == steps);
-      else ns_apply<2, 4, 4><<<na, 512, NS_LDS2, s>>>(g, k & 1, k + 1 == steps);
+      if (w) ns_apply<4, 2, 3><<<na, 512, NS_LDS4, s>>>(g, k & 1, k + 1 == steps, hi_only);
+      else ns_apply<2, 4, 4><<<na, 512, NS_LDS2, s>>>(g, k & 1, k + 1 == steps, hi_only);
     }
     g.count = 0;
     off[w] = 0;
