@@ -43,6 +43,7 @@ __global__ __launch_bounds__(NT) void topk_fwd_kernel(const int* __restrict__ se
         const float* a = E_att + (long)tok * D;
         float acc = 0.f;
         for (int d = 0; d < D; d += 4) {
+#pragma clang fp contract(off)      // products rounded before they are added: which of two near scores is selected hangs on it
           const float4 v = *(const float4*)(a + d);
           acc += v.x * sq[d];
           acc += v.y * sq[d + 1];
