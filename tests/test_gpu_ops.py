@@ -325,6 +325,20 @@ def test_diff_attention_autograd_matches_bwd():
     assert all(torch.equal(a.grad, b) for a, b in zip(leaves, ref))
 
 
+def test_diff_attention_gradient_of_a_sum():
+    """The gradient that arrives is one element for all places (strides of 0)."""
+    import tossctr
+    q, k, v, lam, _ = da_inputs(gen(53), 2, 37, 37, 4, 2, 64, BF)
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    out = tossctr.diff_attention(*leaves, causal=True)
+    out.sum().backward()
+    with torch.no_grad():
+        o, saved = tossctr.diff_attention_fwd(q, k, v, lam, causal=True)
+        want = tossctr.diff_attention_bwd(torch.ones_like(o), q, k, v, lam, o, saved, causal=True)
+    for t, w in zip(leaves, want):
+        assert torch.equal(t.grad, w)
+
+
 def test_diff_attention_gradient_by_differences():
     """dlam and dV are exact differences (the output is linear in them); dQ and dK against central differences of the
     definition in 64 bits, through the bounds of the kernels' gradients."""

@@ -135,3 +135,19 @@ def test_newton_schulz_entry_refusals():
     for c in ((40.0, 0.0, 0.0), (3.0, 3.0, 3.0), (float("nan"), 0.0, 0.0), (2.0, 0.0, 0.0)):
         refuse("coefficients", "ctr_newton_schulz", mats(), 1, 5, *c, 1e-7, 0, P, need, None)
     assert _lib.call("ctr_newton_schulz", None, 0, *ok, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("make,copied", [
+    (lambda: z(2, 5, 3, 2, 32), False),
+    (lambda: z(2, 5, 6, 2, 32)[:, 1:4, ::2], False),
+    (lambda: z(1, 5, 3, 2, 32).expand(4, 5, 3, 2, 32), False),          # one batch for all
+    (lambda: z(2, 5, 3, 2, 64)[..., ::2], True),
+    (lambda: z(2, 5, 3, 2, 33)[..., :32], True),                         # rows off the 16 bytes
+    (lambda: z(1).expand(2, 5, 3, 2, 32), True),                         # the gradient of a sum: one element for all
+    (lambda: z(2, 5, 3, 2, 1).expand(2, 5, 3, 2, 32), True)])
+def test_attention_rows_read_in_place_or_copied(make, copied):
+    from tossctr.ops import _aligned
+    t = make()
+    r, st = _aligned(t)
+    assert (r is not t) == copied and r.shape == t.shape
+    assert r.stride(-1) == 1 and all(s % 8 == 0 for s in st) and list(st) == [s if n > 1 else 0 for s, n in zip(r.stride(), r.shape)][:-1]
