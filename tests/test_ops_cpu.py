@@ -116,6 +116,19 @@ def test_diffattn_entry_workspaces_and_gradients():
     assert _lib.call("ctr_diffattn_fwd", C.byref(attn(B=0)), None, 0, None) == 0
 
 
+def test_diffattn_head_strides_stay_within_32_bit_offsets():
+    """A tile addresses a group's heads by 32-bit byte offsets: 100 heads of 2^23 elements are beyond them, 2 are not."""
+    for heads, st in ((100, 1 << 23), (2, 1 << 30)):
+        refuse("q: 16-byte", "ctr_diffattn_fwd", C.byref(attn(H=heads, Hkv=1, q_sh=st)), P, 0, None)
+        a = attn(H=heads, Hkv=1)
+        refuse("dout", "ctr_diffattn_bwd", C.byref(a), P, 64, 64, st, P, P, P, P, P, 1 << 40, None)
+    refuse("workspace", "ctr_diffattn_bwd", C.byref(attn(H=2, Hkv=1, q_sh=1 << 23)), P, 64, 64, 1 << 23, P, P, P, P, P, 0, None)
+    from tossctr.ops import _aligned
+    t = torch.empty_strided((1, 2, 100, 2, 32), (8, 64, 1 << 23, 32, 1), dtype=BF, device="meta")
+    r, st = _aligned(t)
+    assert r is not t and st[2] == 64
+
+
 def test_newton_schulz_entry_refusals():
     def mats(rows=300, cols=400, ld=400, src=P, dst=P):
         arr = (_lib.NsMat * 1)()

@@ -884,6 +884,9 @@ size_t da_rowstat_bytes(const ctr_diffattn_t* p) {
   return (size_t)p->B * p->Hkv * cdiv((long)p->T * (p->H / p->Hkv), 32) * RS_LINES * 32 * sizeof(float);
 }
 
+// elements from the first to the last head of a group
+long da_span(long sh, long G) { return G == 1 ? 0 : sh > (1L << 40) ? sh : sh * (G - 1); }
+
 int da_check(const ctr_diffattn_t* p, bool bwd) {
   CTR_REQUIRE(p, "null argument");
   CTR_REQUIRE(p->type == TY_BF16 || p->type == TY_F16, "type (1 bf16, 2 fp16)");
@@ -895,15 +898,15 @@ int da_check(const ctr_diffattn_t* p, bool bwd) {
   CTR_REQUIRE(p->scale > 0.f && std::isfinite(p->scale), "scale > 0");
   if ((long)p->B * p->T == 0 && !(bwd && (long)p->B * p->S > 0)) return 0;
   CTR_REQUIRE(p->lam, "null lam");
-  // the row stride is held to what 32 rows' 32-bit byte offsets can reach
+  // a tile's byte offsets are 32 bits wide: those of 32 positions and those of a group's heads are held to 2^30 each
   const auto ok = [](const void* q, std::initializer_list<long> st, long row, long head) {
     if (!q || (uintptr_t)q % 16) return false;
     for (long s : st)
       if (s % 8 || s < 0) return false;
-    return row < (1L << 24) && head < (1L << 24);
+    return row < (1L << 24) && head < (1L << 29);
   };
   const long G = p->H / p->Hkv;
-  CTR_REQUIRE((long)p->B * p->T == 0 || ok(p->q, {p->q_sb, p->q_st, p->q_sh, p->q_sc}, p->q_st, G > 1 ? p->q_sh * std::min(32L, G) / 16 : 0), "q: 16-byte aligned rows");
+  CTR_REQUIRE((long)p->B * p->T == 0 || ok(p->q, {p->q_sb, p->q_st, p->q_sh, p->q_sc}, p->q_st, da_span(p->q_sh, G)), "q: 16-byte aligned rows");
   CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->k, {p->k_sb, p->k_ss, p->k_sh, p->k_sc}, p->k_ss, 0), "k: 16-byte aligned rows");
   CTR_REQUIRE((long)p->B * p->S == 0 || ok(p->v, {p->v_sb, p->v_ss, p->v_sh}, p->v_ss, 0), "v: 16-byte aligned rows");
   CTR_REQUIRE((long)p->B * p->T == 0 || (p->o && (uintptr_t)p->o % 16 == 0 && (uintptr_t)p->o2 % 16 == 0 && (uintptr_t)p->ol % 16 == 0 && !p->o2 == !p->ol), "output");
@@ -1007,7 +1010,7 @@ extern "C" int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long 
   const bool q_on = (long)p->B * p->T > 0, k_on = (long)p->B * p->S > 0;
   CTR_REQUIRE(!q_on || (p->o2 && p->ol && p->stat && dq && dout), "null operand");
   CTR_REQUIRE(!q_on || ((uintptr_t)dout % 16 == 0 && g_sb % 8 == 0 && g_st % 8 == 0 && g_sh % 8 == 0 && g_sb >= 0 &&
-                        g_st >= 0 && g_sh >= 0 && g_st < (1L << 24) && g_sh * (p->H / p->Hkv > 1) < (1L << 24)), "dout: 16-byte aligned rows");
+                        g_st >= 0 && g_sh >= 0 && g_st < (1L << 24) && da_span(g_sh, p->H / p->Hkv) < (1L << 29)), "dout: 16-byte aligned rows");
   CTR_REQUIRE(!k_on || (dk && dv), "null operand");
   CTR_REQUIRE(((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0, "gradients: 16-byte aligned");
   CTR_REQUIRE(ws_bytes >= ctr_diffattn_bwd_ws_size(p), "workspace too small");

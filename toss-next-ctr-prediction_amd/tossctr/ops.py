@@ -162,7 +162,8 @@ def _aligned(t):
     if not t.data_ptr() % 16 and t.is_contiguous() and not (st[0] | st[1] | st[2]) % 8 and st[1] < 1 << 24:
         return t, st[:-1]
     st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    if t.numel() and (t.data_ptr() % 16 or t.stride(-1) != 1 or any(s % 8 or s >= 1 << 24 for s in st[1:-1]) or st[0] % 8):
+    if t.numel() and (t.data_ptr() % 16 or t.stride(-1) != 1 or any(s % 8 or s >= 1 << 24 for s in st[1:-1]) or st[0] % 8 or
+                      st[2] * t.shape[2] >= 1 << 29):
         t = t.clone(memory_format=torch.contiguous_format)
         st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
     return t, st[:-1]
