@@ -259,6 +259,27 @@ def test_diff_attention_lengths(dt, D, causal):
     assert not out[0].any() and not out[2].any() and not dk[1, 1:].any() and not dv[7].any() and not dq[3, 1:].any()
 
 
+@pytest.mark.parametrize("dt,G,D", [(BF, 1, 64), (HF, 2, 32), (BF, 3, 128)])
+def test_diff_attention_rows_that_see_nothing(dt, G, D):
+    """Causal with fewer keys than positions: the first 13 positions see nothing.  NaN in their queries and gradients reaches no
+    one, and NaN in the values that other rows see does not reach them."""
+    import tossctr
+    B, T, S, Hkv = 2, 45, 50, 2
+    q, k, v, lam, do = da_inputs(gen(71 + D), B, T, S, G * Hkv, Hkv, D, dt)
+    lens = torch.tensor([32, 32], device="cuda", dtype=torch.int32)
+    q[:, :13] = 0.0
+    do[:, :13] = 0.0
+    want, want_grads = da_case(q, k, v, lam, do, causal=True, kv_lens=lens)
+    q[:, :13] = math.nan
+    do[:, :13] = math.nan
+    out, saved = tossctr.diff_attention_fwd(q, k, v, lam, causal=True, kv_lens=lens)
+    grads = tossctr.diff_attention_bwd(do, q, k, v, lam, out, saved, causal=True, kv_lens=lens)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+    v[:, :32] = math.nan
+    out, _ = tossctr.diff_attention_fwd(q, k, v, lam, causal=True, kv_lens=lens)
+    assert not out[:, :13].any() and bool(out[:, 13:].isnan().all())
+
+
 def test_diff_attention_large_scores_and_signs():
     """Scores of hundreds (one key takes all), equal maps with lam = 1 (the difference is zero but for roundings), lam of
     either sign, a scale of its own."""

@@ -22,7 +22,7 @@
 // the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.  What
 // the rounding of O left out is kept too: delta_1, taken from the rounded O alone, would add as much again to dQ of short rows.
 #include <algorithm>
-#include <atomic>
+#include <type_traits>
 
 #include "ctr_hip.h"
 #include "vec16.h"
@@ -335,9 +335,10 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
     }
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const bool none = l == 0.f;                  // sees no key: zeros, whatever the keys' values are
+  const float inv = none ? 0.f : 1.f / l;
   if (a.stat && h == 0 && row < a.R)           // a row that sees nothing: +inf, so that its P comes out 0
-    a.stat[map * a.rows + n] = l == 0.f ? INFINITY : fmaf(m, a.c, log2f(l));
+    a.stat[map * a.rows + n] = none ? INFINITY : fmaf(m, a.c, log2f(l));
   // the second map's part goes through LDS to the first map's wave (each path by itself: a value that both change would be
   // copied register by register)
   float* meet = (float*)&tiles[0][0] + pair * DV * 32 + (lane & 31);
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
 #pragma unroll
     for (int j = 0; j < NO; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) meet[(32 * j + c_row(r, h)) * 32] = o[j][r] * inv;
+      for (int r = 0; r < 16; ++r) meet[(32 * j + c_row(r, h)) * 32] = none ? 0.f : o[j][r] * inv;
   }
   __syncthreads();
   if (row >= a.R) return;
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
       for (int r4 = 0; r4 < 4; ++r4) {
         f32x4 x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = o[j][4 * r4 + r] * inv;
+        for (int r = 0; r < 4; ++r) x[r] = none ? 0.f : o[j][4 * r4 + r] * inv;
         put((T*)a.o2 + at, j, r4, x);
       }
   } else {
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
       for (int r4 = 0; r4 < 4; ++r4) {
         f32x4 x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = o[j][4 * r4 + r] * inv - lam * meet[(32 * j + c_row(4 * r4 + r, h)) * 32];
+        for (int r = 0; r < 4; ++r) x[r] = none ? 0.f : o[j][4 * r4 + r] * inv - lam * meet[(32 * j + c_row(4 * r4 + r, h)) * 32];
         put((T*)a.o + at, j, r4, x);
         if (a.ol) {
 #pragma unroll
@@ -663,7 +664,9 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
   const int kb = tile * 32 * NP, kw = kb + pair * 32, key = kw + (lane & 31), kr = min(key, a.S - 1);
   // rows that see a key of the block: positions from t0 to the sequence's end
   const int t0 = kb >= s.kl ? s.ql : a.causal ? max(0, kb - (s.kl - s.ql)) : 0;
-  int r0 = t0 * a.G / 32 * 32, r1 = s.ql * a.G;
+  // (rows of the first tile before t0 come as zeros: a row that sees no key adds nothing, whatever its dO holds)
+  const int r_lo = t0 * a.G;
+  int r0 = r_lo / 32 * 32, r1 = s.ql * a.G;
   if (a.splits > 1) {              // this split's share of them
     const int per = (max(0, r1 - r0) / 32 + a.splits) / a.splits * 32;
     r0 += sp * per;
@@ -674,7 +677,7 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
   int tb = r0 / a.G, rem = r0 - tb * a.G;
   const uint32_t magic = a.G == 1 ? 0 : (uint32_t)((0x100000000ull + a.G - 1) / a.G);
   const auto over_g = [&](int n) { return a.G == 1 ? n : (int)__umulhi((uint32_t)n, magic); };
-  const auto stage = [&](int rb, int cur) {
+  const auto stage = [&](int rb, int cur, auto first) {
     const auto qb = (const T*)a.q + s.b * a.q_sb + tb * a.q_st + s.hk * a.G * a.q_sh;
     const auto gb = (const T*)a.dout + s.b * a.g_sb + tb * a.g_st + s.hk * a.G * a.g_sh;
 #pragma unroll
@@ -686,7 +689,9 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
       for (int j = 0; j < St::PER; ++j) {
         const int x = plan.row[i] + j * step, t = over_g(rem + x), g = rem + x - t * a.G;
         const uint32_t off = t * st + g * sh + plan.byte[i][j];
-        dma16(rs, tiles[cur] + St::place(role, wave) + j * 512, rb + x < r1 ? off : BUF_OOB);
+        bool in = rb + x < r1;
+        if constexpr (decltype(first)::value) in = in && rb + x >= r_lo;
+        dma16(rs, tiles[cur] + St::place(role, wave) + j * 512, in ? off : BUF_OOB);
       }
     }
     rem += 32;
@@ -695,7 +700,7 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
     rem -= t * a.G;
     if (wave == 0) dma16(open_range(a.part + ((long)bh * a.tiles32 + rb / 32) * (RS_LINES * 32)), stats[cur], lane * 16);
   };
-  if (r0 < r1) stage(r0, 0);
+  if (r0 < r1) stage(r0, 0, std::true_type());
   const long out = ((long)s.b * a.S + key) * a.Hkv + s.hk;
   // four elements of the key's dK (from 0) or dV (from DV), or of their part
   const auto put = [&](T* to, int from, int c, const f32x4& x) {
@@ -717,7 +722,7 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
     int cur = 0;
     for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
       tile_ready();
-      if (rb + 32 < r1) stage(rb + 32, cur ^ 1);
+      if (rb + 32 < r1) stage(rb + 32, cur ^ 1, std::false_type());
       const T* qs = tiles[cur];
       const float* st = stats[cur];
       // a row below the diagonal of the pair's last key, or a key behind the end, needs the mask
@@ -789,7 +794,7 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
     int cur = 0;
     for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
       tile_ready();
-      if (rb + 32 < r1) stage(rb + 32, cur ^ 1);
+      if (rb + 32 < r1) stage(rb + 32, cur ^ 1, std::false_type());
       const T* gs = tiles[cur] + 64 * D;
       const float* st = stats[cur];
       f32x16 dp = 0.f;
