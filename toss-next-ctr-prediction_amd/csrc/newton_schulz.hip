@@ -682,16 +682,29 @@ bool ns_large_dims(NsMat& q) {
   return true;
 }
 
-// the largest singular value that X can reach, and W: the polynomial scanned over [0, r] each step
+// The largest singular value r that X can reach, and W: with u the square of one, W's is p(u) = a + b u + c u^2 and X's next
+// sqrt(u) p(u); over [0, r^2] both are largest at an end or where 2 c u + b = 0, 5 c u^2 + 3 b u + a = 0.
 bool ns_in_range(int steps, double a, double b, double c) {
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-  double r = 1.0;
+  const auto p = [=](double u) { return std::fabs(a + u * (b + u * c)); };
+  double at[5] = {0., 0., -1., -1., -1.};
+  if (c != 0.) {
+    at[2] = -b / (2. * c);
+    const double d = 9. * b * b - 20. * a * c;
+    if (d >= 0.) {
+      const double q = -0.5 * (3. * b + std::copysign(std::sqrt(d), b));      // the roots q / (5 c) and a / q, without cancelling
+      at[3] = q / (5. * c);
+      if (q != 0.) at[4] = a / q;
+    }
+  } else if (b != 0.) at[3] = -a / (3. * b);
+  double r = 1.;
   for (int s = 0; s < steps; ++s) {
-    double next = 0., w = 0.;
-    for (int i = 0; i <= 4096; ++i) {
-      const double v = r * i / 4096, v2 = v * v, pv = std::fabs(a + b * v2 + c * v2 * v2);
-      w = std::max(w, pv);
-      next = std::max(next, v * pv);
+    at[1] = r * r;
+    double w = 0., next = 0.;
+    for (const double u : at) {
+      if (!(u >= 0. && u <= r * r)) continue;
+      w = std::max(w, p(u));
+      next = std::max(next, std::sqrt(u) * p(u));
     }
     if (!(w <= 32.) || !(next <= 7.5)) return false;
     r = next * 1.001;
