@@ -264,8 +264,10 @@ __global__ __launch_bounds__(1024) void ln_reduce(const float* __restrict__ part
   if (!out) return;
   const float* p = part + (long)blockIdx.y * np * N;
   float v = 0.f;
-  if (c < N)
+  if (c < N) {
+#pragma unroll 16                 // as many loads in flight
     for (int i = r; i < np; i += 32) v += p[(long)i * N + c];
+  }
   s[r][cl] = v;
   __syncthreads();
   for (int o = 16; o > 0; o >>= 1) {
