@@ -416,6 +416,11 @@ def test_newton_schulz(shapes, dt):
     assert all(torch.equal(a, b) for a, b in zip(out, tossctr.newton_schulz(mats)))
 
 
+@pytest.mark.parametrize("shapes,dt", [([(801, 900), (1100, 770)], F32), ([(790, 12161)], F32), ([(12200, 771), (33, 70)], BF)])
+def test_newton_schulz_large_tiles(shapes, dt):
+    test_newton_schulz(shapes, dt)
+
+
 def test_newton_schulz_forms():
     """Batches, strides, transposes, one step, other coefficients, zeros, sizes of 1e30 and 1e-30."""
     import tossctr

@@ -21,7 +21,7 @@ namespace {
 
 constexpr float SX = 4096.f, SA = 1024.f;      // the planes' scales of X and of A, W
 constexpr int NS_MAXMAT = 20;                  // matrices of one launch (their table rides in the kernel arguments)
-constexpr int NS_TILE = 128, NS_BK = 32;
+constexpr int NS_BK = 32;
 constexpr int NS_SUMSQ_BLOCKS = 256;
 constexpr int NS_SMALL_LDS = 160 * 1024 - 256;   // of a workgroup, next to its few static bytes
 
@@ -32,7 +32,7 @@ struct NsMat {
   int rows, cols;          // as given
   int m, n, mp, np;        // m <= n, and both rounded up to the tile
   long off_x, off_a, off_p, off_s;     // bytes into the workspace: X planes (two buffers), A and W planes, partials, sums
-  int splits, asplits, type, wr;      // shares of K of X X^T and of A A; the tile rows in 64s
+  int splits, asplits, type, group;      // shares of K of X X^T and of A A
  
 };
 struct NsArgs {
@@ -176,42 +176,56 @@ __device__ __forceinline__ void ns_wait() {      // all but the last N loads hav
   asm volatile("" ::: "memory");
 }
 
-// A tile of 64 WR x 128 of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.
-// WR CW = 8 waves of 64 x 128 / CW, two a SIMD: one's products run under the other's LDS reads (four waves of 64 x 64 took
-// 0.86 us a step, the sum of both).  A K step's four planes come by direct loads to one of NST places in LDS, NST - 1 steps
-// ahead -- a step's products last shorter than a load, so one is not enough: 256 x 128 (WR = 4) and three places for large
-// matrices, where the larger tile reads a quarter less, 128 x 128 and four places where a tile's chain of steps is what
-// counts.  In LDS a row of 128 bytes (A, NT: hi and lo of 32 k) holds its 16-byte chunk c at c ^ (row / 2 % 8), one of 512
-// bytes (NN: hi and lo of 128 columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads cover all banks.
-template <int WR> constexpr int ns_stage() { return 2 * NS_BK * (64 * WR + NS_TILE); }      // elements of a step's planes
-template <bool NN, int WR, int CW, int NST>
+// A tile of a product, K from k0 to k1 (multiples of 32): A rows from r0, B rows (NT) or columns (NN) from c0.  Eight waves, WR
+// by 8 / WR, of NI x NJ blocks of 32 x 32: two a SIMD, so that one's products run under the other's LDS reads (four waves of
+// 64 x 64 took the sum of both, 0.86 us a step).  A K step's planes come by direct loads to one of NST places in LDS, NST - 1
+// steps ahead.  2048 x 2048 x 8192, three products: 256 x 256 tiles 186 us (1.1 PFLOP/s, the rate of a large 16-bit product on
+// this card is 1.25), 256 x 128 197; its symmetric product, with half as many tiles: 256 x 128 150, 256 x 256 165; below 768
+// rows, where a tile's chain of steps is what counts, 128 x 128 (512 x 7552: 20 us, 0.6 PFLOP/s).
+// In LDS a row of 128 bytes (A, NT: hi and lo of 32 k) holds its 16-byte chunk c at c ^ (row / 2 % 8), one of 4 C bytes (NN:
+// hi and lo of C columns) at c ^ (4 (row % 4) + row / 4 % 4): the row and the transpose reads cover all banks.
+template <int WR_, int NI_, int NJ_, int NST_>
+struct NsTile {
+  static constexpr int WR = WR_, WC = 8 / WR, NI = NI_, NJ = NJ_, NST = NST_, R = 32 * WR * NI, C = 32 * WC * NJ;
+  static constexpr int PA = 2 * NS_BK * R, STAGE = 2 * NS_BK * (R + C);      // elements of a step's planes of A, of both
+  static constexpr int LDS = std::max(NST * STAGE, 2 * 128 * (C + 8)) * 2;   // bytes, the store of the result included
+  using Acc = f32x16[NI][NJ];
+};
+constexpr int NS_GROUPS = 3;               // matrices that share their tiles
+using NsSmall = NsTile<2, 2, 1, 4>;        // 128 x 128
+using NsMid = NsTile<4, 2, 2, 3>;          // 256 x 128
+using NsLarge = NsTile<2, 4, 2, 2>;        // 256 x 256
+template <bool NN, class S>
 __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float16* B, int ldb, int r0, int c0, int k0, int k1,
-                                        _Float16* lds, bool hi_only, f32x16 (&acc)[2][4 / CW]) {
-  static_assert(WR * CW == 8, "eight waves deal out the loads");
-  constexpr int PA = 2 * 64 * WR * NS_BK, STAGE = ns_stage<WR>(), NJ = 4 / CW, LOADS = WR + 2;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / CW * 64, wc = wave % CW * (NS_TILE / CW);
+                                        _Float16* lds, bool hi_only, typename S::Acc& acc) {
+  constexpr int NI = S::NI, NJ = S::NJ, NST = S::NST, NA = S::R / 64, NB = S::C / 64, LOADS = NA + NB, RPL = 256 / S::C;
+  static_assert(S::R % 128 == 0 && (S::C == 128 || S::C == 256), "loads dealt to eight waves");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave / S::WC * 32 * NI, wc = wave % S::WC * 32 * NJ;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
-  // a load is 8 rows of 128 bytes, or 2 of 512; wave w takes WR of A and two of B
-  const _Float16* asrc = A + at(r0 + 8 * WR * wave, k0, lda);
-  const _Float16* bsrc = B + (NN ? at(k0 + 4 * wave, c0, ldb) : at(c0 + 16 * wave, k0, ldb));
-  uint32_t aoff[2], boff[2];
+  // a load is 8 rows of 128 bytes, or RPL of 4 C; a wave takes NA of A and NB of B
+  const _Float16* asrc = A + at(r0 + 8 * NA * wave, k0, lda);
+  const _Float16* bsrc = B + (NN ? at(k0 + 4 * wave, c0, ldb) : at(c0 + 8 * NB * wave, k0, ldb));
+  uint32_t aoff[2], boff[NB];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    aoff[j] = (lane >> 3) * lda * 4 + ((lane & 7) ^ ((4 * (WR * wave + j) + (lane >> 4)) & 7)) * 16;
-    boff[j] = NN ? (lane >> 5) * ldb * 4 + ((lane & 31) ^ ((((2 * j + (lane >> 5)) & 3) << 2) | (wave & 3))) * 16
+  for (int j = 0; j < 2; ++j) aoff[j] = (lane >> 3) * lda * 4 + ((lane & 7) ^ ((4 * j + (lane >> 4)) & 7)) * 16;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int r = RPL * j + lane / (S::C / 4);        // of the wave's four K rows
+    boff[j] = NN ? lane / (S::C / 4) * ldb * 4 + ((lane % (S::C / 4)) ^ ((r & 3) << 2 | (wave & 3))) * 16
                  : (lane >> 3) * ldb * 4 + ((lane & 7) ^ ((4 * j + (lane >> 4)) & 7)) * 16;
   }
   const auto stage = [&](int step, int place) {
     const auto ra = buf_rsrc(asrc + (long)step * 2 * NS_BK, 0x7ffffff0u);
     const auto rb = buf_rsrc(bsrc + (NN ? (long)step * 2 * NS_BK * ldb : (long)step * 2 * NS_BK), 0x7ffffff0u);
-    const uint32_t ta = lds0 + (place * STAGE + wave * WR * 512) * 2, tb = lds0 + (place * STAGE + PA + wave * 1024) * 2;
+    const uint32_t ta = lds0 + (place * S::STAGE + wave * NA * 512) * 2, tb = lds0 + (place * S::STAGE + S::PA + wave * NB * 512) * 2;
 #pragma unroll
-    for (int j = 0; j < WR; ++j) ns_dma16(ra, ta + j * 1024, aoff[j & 1], j * 32 * lda);
+    for (int j = 0; j < NA; ++j) ns_dma16(ra, ta + j * 1024, aoff[j & 1], j * 32 * lda);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) ns_dma16(rb, tb + j * 1024, boff[j], j * (NN ? 8 : 32) * ldb);
+    for (int j = 0; j < NB; ++j) ns_dma16(rb, tb + j * 1024, boff[j], j * (NN ? 4 * RPL : 32) * ldb);
   };
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = 0.f;
   const int steps = (k1 - k0) / NS_BK;
@@ -221,16 +235,16 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float
   const int row = lane & 31, h = lane >> 5, turn = (row >> 1) & 7;
   const int arow = (wr + row) * 2 * NS_BK, brow = (wc + row) * 2 * NS_BK;
   const int tk = 8 * h + ((lane & 15) >> 2), tc = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;      // transpose reads: row, column
-  struct Frags { f16x8 a[2][2], b[2][NJ]; };      // [plane][tile]
+  struct Frags { f16x8 a[2][NI], b[2][NJ]; };      // [plane][tile]
   const auto read = [&](int place, int kk) {
-    const _Float16* s = lds + place * STAGE;
-    const _Float16* bp = s + PA;
+    const _Float16* s = lds + place * S::STAGE;
+    const _Float16* bp = s + S::PA;
     Frags f;
 #pragma unroll
     for (int pl = 0; pl < 2; ++pl) {
       const int ch = ((4 * pl + 2 * kk + h) ^ turn) * 8;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) f.a[pl][i] = *(const f16x8*)(s + arow + 64 * i * NS_BK + ch);
+      for (int i = 0; i < NI; ++i) f.a[pl][i] = *(const f16x8*)(s + arow + 64 * i * NS_BK + ch);
 #pragma unroll
       for (int i = 0; i < NJ; ++i) {
         if constexpr (!NN) f.b[pl][i] = *(const f16x8*)(bp + brow + 64 * i * NS_BK + ch);
@@ -239,7 +253,7 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int r = 16 * kk + tk + 4 * half, c = (wc / 32 + i) * 8 + 4 * pl + (tc >> 3);
-            const _Float16* q = bp + r * 2 * NS_TILE + (c ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (tc & 4);
+            const _Float16* q = bp + r * 2 * S::C + (c ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (tc & 4);
             u[half] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
           }
           f.b[pl][i] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -253,29 +267,71 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float
     for (int pr = 0; pr < 3; ++pr) {    // lo hi, hi lo, hi hi; the accumulators in turn
       if (pr < 2 && hi_only) continue;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = MFMA16(f.a[pr == 0][i], f.b[pr == 1][j], acc[i][j]);
     }
   };
-  // Half a step's fragments are read while the half before is multiplied; the barrier, in the middle of a step, is where the
-  // next one has landed and the place of the last one is free.
-  if (steps <= 0) return;
-  if (steps >= NST - 1) ns_wait<LOADS * (NST - 2)>();
-  else ns_wait<0>();
-  Frags f = read(0, 0);
   int place = 0;
-  for (int k = 0; k < steps; ++k) {
-    const Frags g = read(place, 1);
-    multiply(f);
-    if (k + 1 < steps) {
-      if (k + NST - 1 <= steps) ns_wait<LOADS * (NST - 3)>();
+  if constexpr (NI * NJ > 4) {      // no registers for a second set of fragments; written out, as read() and multiply() spill here
+    for (int k = 0; k < steps; ++k) {
+      if (k + NST - 1 <= steps) ns_wait<LOADS * (NST - 2)>();
       else ns_wait<0>();
       if (k + NST - 1 < steps) stage(k + NST - 1, place == 0 ? NST - 1 : place - 1);
+      const _Float16* s = lds + place * S::STAGE;
+      const _Float16* bp = s + S::PA;
       place = place + 1 == NST ? 0 : place + 1;
-      f = read(place, 0);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        f16x8 fa[2][NI], fb[2][NJ];
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl) {
+          const int ch = ((4 * pl + 2 * kk + h) ^ turn) * 8;
+#pragma unroll
+          for (int i = 0; i < NI; ++i) fa[pl][i] = *(const f16x8*)(s + arow + 64 * i * NS_BK + ch);
+#pragma unroll
+          for (int i = 0; i < NJ; ++i) {
+            if constexpr (!NN) fb[pl][i] = *(const f16x8*)(bp + brow + 64 * i * NS_BK + ch);
+            else {
+              f16x4 u[2];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const int r = 16 * kk + tk + 4 * half, c = (wc / 32 + i) * 8 + 4 * pl + (tc >> 3);
+                const _Float16* q = bp + r * 2 * S::C + (c ^ (((r & 3) << 2) | ((r >> 2) & 3))) * 8 + (tc & 4);
+                u[half] = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
+              }
+              fb[pl][i] = __builtin_shufflevector(u[0], u[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+          }
+        }
+#pragma unroll
+        for (int pr = 0; pr < 3; ++pr) {
+          if (pr < 2 && hi_only) continue;
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = MFMA16(fa[pr == 0][i], fb[pr == 1][j], acc[i][j]);
+        }
+      }
     }
-    multiply(g);
+  } else {
+    // Half a step's fragments are read while the half before is multiplied; the barrier, in the middle of a step, is where the
+    // next one has landed and the place of the last one is free.
+    if (steps >= NST - 1) ns_wait<LOADS * (NST - 2)>();
+    else ns_wait<0>();
+    Frags f = read(0, 0);
+    for (int k = 0; k < steps; ++k) {
+      const Frags g = read(place, 1);
+      multiply(f);
+      if (k + 1 < steps) {
+        if (k + NST - 1 <= steps) ns_wait<LOADS * (NST - 3)>();
+        else ns_wait<0>();
+        if (k + NST - 1 < steps) stage(k + NST - 1, place == 0 ? NST - 1 : place - 1);
+        place = place + 1 == NST ? 0 : place + 1;
+        f = read(place, 0);
+      }
+      multiply(g);
+    }
   }
 }
 
@@ -287,48 +343,41 @@ __device__ __forceinline__ void tri(int id, int& ti, int& tj) {
   tj = id - ti * (ti + 1) / 2;
 }
 
-// tiles of 64 WR x 128 that meet the lower triangle, row by row
-template <int WR>
+// tiles of S that meet the lower triangle, row by row
+template <class S>
 __device__ __forceinline__ void tri_tile(int id, int& ti, int& tj) {
-  if constexpr (WR == 2) tri(id, ti, tj);
-  else {
-    tri(id >> 1, ti, tj);       // row ti has 2 (ti + 1) of them
-    tj = 2 * tj + (id & 1);
-  }
+  constexpr int W = S::R / S::C;
+  tri(id / W, ti, tj);       // row ti has W (ti + 1) of them
+  tj = W * tj + id % W;
 }
-__host__ __device__ inline int tri_tiles(int mp, int wr) {
-  const int n = mp / (64 * wr);
-  return n * (n + 1) / 2 * (wr == 2 ? 1 : 2);
-}
+template <class S>
+__host__ __device__ inline int tri_tiles(int mp) { return mp / S::R * (mp / S::R + 1) / 2 * (S::R / S::C); }
 
 // partials of X X^T (square = false) or A A over a share of K, lower tiles; the workgroups of an XCD (every eighth) take the
 // same share, whose rows so stay in its L2
-template <int WR, int CW, int NST>
-__global__ __launch_bounds__(64 * WR * CW, 1) void ns_gram(const NsArgs p, int buf, bool square, bool hi_only) {
+template <class S>
+__global__ __launch_bounds__(512, 2) void ns_gram(const NsArgs p, int buf, bool square, bool hi_only) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
   const int splits = square ? q.asplits : q.splits, id = blockIdx.x - p.pre[i], K = square ? q.mp : q.np;
-  const int tiles = tri_tiles(q.mp, WR), sp = (id >> 3) / tiles * 8 + (id & 7);
+  const int tiles = tri_tiles<S>(q.mp), sp = (id >> 3) / tiles * 8 + (id & 7);
   if (sp >= splits) return;
   int ti, tj;
-  tri_tile<WR>((id >> 3) % tiles, ti, tj);
+  tri_tile<S>((id >> 3) % tiles, ti, tj);
   const int steps = K / NS_BK, per = (steps + splits - 1) / splits;
   const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + (long)buf * 2 * q.mp * K;
-  constexpr int NJ = 4 / CW;
-  f32x16 acc[2][NJ];
-  ns_tile<false, WR, CW, NST>(x, K, x, K, ti * 64 * WR, tj * NS_TILE, min(steps, sp * per) * NS_BK,
-                      min(steps, (sp + 1) * per) * NS_BK, lds, hi_only, acc);
+  typename S::Acc acc;
+  ns_tile<false, S>(x, K, x, K, ti * S::R, tj * S::C, min(steps, sp * per) * NS_BK, min(steps, (sp + 1) * per) * NS_BK, lds, hi_only, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC * 32 * S::NI, wc = wave % S::WC * 32 * S::NJ;
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int a = 0; a < S::NI; ++a)
 #pragma unroll
-    for (int b = 0; b < NJ; ++b)
+    for (int b = 0; b < S::NJ; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        out[(long)(ti * 64 * WR + wave / CW * 64 + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * NS_TILE +
-            wave % CW * (NS_TILE / CW) + b * 32 + (lane & 31)] = acc[a][b][r];
+        out[(long)(ti * S::R + wr + a * 32 + c_row(r, lane >> 5)) * q.mp + tj * S::C + wc + b * 32 + (lane & 31)] = acc[a][b][r];
 }
 
 // the partials of a 32 x 32 block of the lower tiles summed in order (four elements a thread, eight loads in flight), and A
@@ -389,54 +438,58 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
 
 // X' = W X; the last step writes the result in its own type and orientation.  An XCD takes every eighth panel of columns, with
 // all row tiles of one together.
-template <int WR, int CW, int NST>
-__global__ __launch_bounds__(64 * WR * CW, 1) void ns_apply(const NsArgs p, int buf, int last, bool hi_only) {
+template <class S>
+__global__ __launch_bounds__(512, 2) void ns_apply(const NsArgs p, int buf, int last, bool hi_only) {
   extern __shared__ __align__(16) _Float16 lds[];
+  constexpr int NI = S::NI, NJ = S::NJ;
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
-  const int id = blockIdx.x - p.pre[i], mt = q.mp / (64 * WR), r0 = (id >> 3) % mt * 64 * WR, c0 = ((id >> 3) / mt * 8 + (id & 7)) * NS_TILE;
+  const int id = blockIdx.x - p.pre[i], mt = q.mp / S::R, r0 = (id >> 3) % mt * S::R, c0 = ((id >> 3) / mt * 8 + (id & 7)) * S::C;
   if (c0 >= q.np) return;
-  const long plane = (long)q.mp * q.np, planeW = (long)q.mp * q.mp;
-  const _Float16* W = (const _Float16*)(p.ws + q.off_a) + 2 * planeW;
-  const _Float16* x = (const _Float16*)(p.ws + q.off_x) + buf * 2 * plane;
-  _Float16* y = (_Float16*)(p.ws + q.off_x) + (buf ^ 1) * 2 * plane;
-  constexpr int NJ = 4 / CW;
-  f32x16 acc[2][NJ];
-  ns_tile<true, WR, CW, NST>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, hi_only, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const _Float16* W = (const _Float16*)(p.ws + q.off_a) + 2 * (long)q.mp * q.mp;
+  const _Float16* x = (const _Float16*)(p.ws + q.off_x) + (long)buf * 2 * q.mp * q.np;
+  _Float16* y = (_Float16*)(p.ws + q.off_x) + (long)(buf ^ 1) * 2 * q.mp * q.np;
+  typename S::Acc acc;
+  ns_tile<true, S>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, hi_only, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC * 32 * NI, wc = wave % S::WC * 32 * NJ;
   const bool tall = q.rows > q.cols;
   if (last) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < NI; ++a)
 #pragma unroll
       for (int b = 0; b < NJ; ++b) {
-        const int c = c0 + wave % CW * (NS_TILE / CW) + b * 32 + (lane & 31);
+        const int c = c0 + wc + b * 32 + (lane & 31);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int row = r0 + wave / CW * 64 + a * 32 + c_row(r, lane >> 5);
+          const int row = r0 + wr + a * 32 + c_row(r, lane >> 5);
           if (row < q.m && c < q.n) ns_store(q, tall ? c : row, tall ? row : c, acc[a][b][r] * (1.f / (SA * SX)));
         }
       }
     return;
   }
-  // the planes go out through LDS, 16 bytes a lane along a row
-  constexpr int LD = NS_TILE + 8, PL = 64 * WR * LD;
-  __syncthreads();
+  // the planes go out through LDS, 128 rows at a time, 16 bytes a lane along a row
+  constexpr int LD = S::C + 8, PL = 128 * LD, CPR = S::C / 8;
+  static_assert(128 % (32 * NI) == 0, "a wave's rows lie in one pass");
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int pass = 0; pass < S::R / 128; ++pass) {
+    __syncthreads();
+    if (wr / 128 == pass) {
 #pragma unroll
-    for (int b = 0; b < NJ; ++b)
+      for (int a = 0; a < NI; ++a)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int o = (wave / CW * 64 + a * 32 + c_row(r, lane >> 5)) * LD + wave % CW * (NS_TILE / CW) + b * 32 + (lane & 31);
-        split16(acc[a][b][r] * (1.f / SA), lds[o], lds[PL + o]);
-      }
-  __syncthreads();
-  constexpr int PER = 2 * 64 * WR * (NS_TILE / 8) / (64 * WR * CW);
+        for (int b = 0; b < NJ; ++b)
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int e = threadIdx.x + k * 64 * WR * CW, c = e % (NS_TILE / 8), row = e / (NS_TILE / 8) % (64 * WR), pl = e / (NS_TILE / 8) / (64 * WR);
-    *(f16x8*)(y + at(r0 + row, c0 + c * 8, q.np) + pl * 32) = *(const f16x8*)(lds + pl * PL + row * LD + c * 8);
+          for (int r = 0; r < 16; ++r) {
+            const int o = (wr % 128 + a * 32 + c_row(r, lane >> 5)) * LD + wc + b * 32 + (lane & 31);
+            split16(acc[a][b][r] * (1.f / SA), lds[o], lds[PL + o]);
+          }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2 * 128 * CPR / 512; ++k) {
+      const int e = threadIdx.x + k * 512, c = e % CPR, row = e / CPR % 128, pl = e / CPR / 128;
+      *(f16x8*)(y + at(r0 + pass * 128 + row, c0 + c * 8, q.np) + pl * 32) = *(const f16x8*)(lds + pl * PL + row * LD + c * 8);
+    }
   }
 }
 
@@ -672,11 +725,12 @@ int ns_splits(int tiles, int K) {
 
 bool ns_large_dims(NsMat& q) {
   if (ns_is_small(q.mp, q.np)) return false;
-  q.wr = q.m > 768 ? 4 : 2;
-  q.mp = cdiv(q.m, 64 * q.wr) * 64 * q.wr;
-  q.np = cdiv(q.n, NS_TILE) * NS_TILE;
-  if (q.np < q.mp) q.np = q.mp;
-  const int tiles = tri_tiles(q.mp, q.wr);
+  // 256 x 256 tiles where they are three for every four compute units or more
+  q.group = q.m <= 768 ? 0 : (long)cdiv(q.m, 256) * cdiv(q.n, 256) < 192 ? 1 : 2;
+  const int r = q.group ? 256 : 128, c = q.group == 2 ? 256 : 128;
+  q.mp = cdiv(q.m, r) * r;
+  q.np = std::max(cdiv(q.n, c) * c, q.mp);
+  const int tiles = q.group ? tri_tiles<NsMid>(q.mp) : tri_tiles<NsSmall>(q.mp);
   q.splits = ns_splits(tiles, q.np);
   q.asplits = ns_splits(tiles, q.mp);
   return true;
@@ -712,9 +766,6 @@ bool ns_in_range(int steps, double a, double b, double c) {
   return true;
 }
 
-constexpr int NS_LDS4 = 3 * ns_stage<4>() * (int)sizeof(_Float16), NS_LDS2 = 4 * ns_stage<2>() * (int)sizeof(_Float16);
-static_assert(2 * 256 * (NS_TILE + 8) * 2 <= NS_LDS4 && 2 * 128 * (NS_TILE + 8) * 2 <= NS_LDS2, "the result's planes take the K steps' place");
-
 // the kernels' LDS beyond 64 KB, once for each device
 bool ns_allow_lds() {
   static std::atomic<uint64_t> done{0};
@@ -725,8 +776,9 @@ bool ns_allow_lds() {
   const auto allow = [](const void* f, int n) {
     return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n) == hipSuccess;
   };
-  if (!allow((const void*)ns_gram<4, 2, 3>, NS_LDS4) || !allow((const void*)ns_gram<2, 4, 4>, NS_LDS2) ||
-      !allow((const void*)ns_apply<4, 2, 3>, NS_LDS4) || !allow((const void*)ns_apply<2, 4, 4>, NS_LDS2) ||
+  if (!allow((const void*)ns_gram<NsSmall>, NsSmall::LDS) || !allow((const void*)ns_apply<NsSmall>, NsSmall::LDS) ||
+      !allow((const void*)ns_gram<NsMid>, NsMid::LDS) || !allow((const void*)ns_apply<NsMid>, NsMid::LDS) ||
+      !allow((const void*)ns_apply<NsLarge>, NsLarge::LDS) ||
       !allow((const void*)ns_small<float>, NS_SMALL_LDS) ||
       !allow((const void*)ns_small<__bf16>, NS_SMALL_LDS) || !allow((const void*)ns_small<_Float16>, NS_SMALL_LDS))
     return false;
@@ -740,14 +792,14 @@ bool ns_allow_lds() {
 using namespace ctr;
 
 extern "C" size_t ctr_newton_schulz_ws_size(const ctr_ns_mat_t* mats, int count) {
-  size_t most = 0, off[2] = {0, 0};
-  int in[2] = {0, 0};
+  size_t most = 0, off[NS_GROUPS] = {};
+  int in[NS_GROUPS] = {};
   for (int i = 0; mats && i < count; ++i) {
     if (mats[i].rows <= 0 || mats[i].cols <= 0) continue;
     NsMat q;
     ns_dims(q, mats[i], 0);
     if (!ns_large_dims(q)) continue;
-    const int g = q.wr == 4;
+    const int g = q.group;
     if (in[g] == NS_MAXMAT) in[g] = 0, off[g] = 0;
     off[g] = ns_layout(q, off[g]);
     ++in[g];
@@ -787,8 +839,8 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     ns = 0;
     small_lds = 0;
   };
-  NsArgs large[2] = {};             // by their tile
-  size_t off[2] = {0, 0};
+  NsArgs large[NS_GROUPS] = {};
+  size_t off[NS_GROUPS] = {};
   for (NsArgs& g : large) {
     g.ws = (char*)ws;
     g.a = a;
@@ -816,15 +868,17 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
       // whose roundings, 2^-12 of each operand, add a twentieth to the result's own error
       const bool hi_only = k + 1 == steps && steps > 1 && type == TY_BF16;
       for (int square = 0; square < 2; ++square) {
-        const int ng = prefix([&](const NsMat& q) { return cdiv(square ? q.asplits : q.splits, 8) * 8 * tri_tiles(q.mp, q.wr); });
-        if (w) ns_gram<4, 2, 3><<<ng, 512, NS_LDS4, s>>>(g, k & 1, square, hi_only);
-        else ns_gram<2, 4, 4><<<ng, 512, NS_LDS2, s>>>(g, k & 1, square, hi_only);
+        const int ng = prefix([&](const NsMat& q) { return cdiv(square ? q.asplits : q.splits, 8) * 8 * (w ? tri_tiles<NsMid>(q.mp) : tri_tiles<NsSmall>(q.mp)); });
+        if (w) ns_gram<NsMid><<<ng, 512, NsMid::LDS, s>>>(g, k & 1, square, hi_only);
+        else ns_gram<NsSmall><<<ng, 512, NsSmall::LDS, s>>>(g, k & 1, square, hi_only);
         const int nj = prefix([](const NsMat& q) { return (q.mp / 32) * (q.mp / 32 + 1) / 2; });
         ns_join<<<nj, 256, 0, s>>>(g, square);
       }
-      const int na = prefix([](const NsMat& q) { return q.mp / (64 * q.wr) * (cdiv(q.np / NS_TILE, 8) * 8); });
-      if (w) ns_apply<4, 2, 3><<<na, 512, NS_LDS4, s>>>(g, k & 1, k + 1 == steps, hi_only);
-      else ns_apply<2, 4, 4><<<na, 512, NS_LDS2, s>>>(g, k & 1, k + 1 == steps, hi_only);
+      const int tr = w ? 256 : 128, tc = w == 2 ? 256 : 128;
+      const int na = prefix([&](const NsMat& q) { return q.mp / tr * (cdiv(q.np / tc, 8) * 8); });
+      if (w == 2) ns_apply<NsLarge><<<na, 512, NsLarge::LDS, s>>>(g, k & 1, k + 1 == steps, hi_only);
+      else if (w) ns_apply<NsMid><<<na, 512, NsMid::LDS, s>>>(g, k & 1, k + 1 == steps, hi_only);
+      else ns_apply<NsSmall><<<na, 512, NsSmall::LDS, s>>>(g, k & 1, k + 1 == steps, hi_only);
     }
     g.count = 0;
     off[w] = 0;
@@ -834,7 +888,7 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     NsMat q;
     ns_dims(q, mats[i], type);
     if (ns_large_dims(q)) {
-      const int w = q.wr == 4;
+      const int w = q.group;
       if (large[w].count == NS_MAXMAT) flush_large(w);
       off[w] = ns_layout(q, off[w]);
       large[w].mat[large[w].count++] = q;
@@ -845,8 +899,7 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     }
   }
   flush_small();
-  flush_large(0);
-  flush_large(1);
+  for (int w = 0; w < NS_GROUPS; ++w) flush_large(w);
   return check_launch("newton_schulz");
 }
 
