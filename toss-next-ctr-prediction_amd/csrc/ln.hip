@@ -11,7 +11,7 @@
 // a wave and a wide one never spills.  Rows beyond 16384 elements stream (ln_*_wide).
 // Measured: 32768 x 4096 bf16 forward 134 us (4.0 TB/s), backward with the join 168 us (4.8 TB/s), a large copy reaching 4.65;
 // 245760 x 32 bf16 9 and 13 + 4 us (3.5 and 3.6 TB/s); 4099 x 1001 fp16, every row at another alignment, 7.2 us (2.3 TB/s).
-// Small calls (64 x 256: 3.7 + 4.9 + 2.8 us of kernels) are bound by the launches and the host (26 us).
+// Small calls (64 x 256: forward and backward in two launches, 23 us) are bound by the host.
 // Weight gradients: a thread keeps its columns' sums over all rows of its block in registers, the block joins its
 // row groups in a fixed order and writes one partial row, ln_reduce adds the partial rows in a fixed order: no atomics,
 // the same bits every time.
@@ -292,6 +292,9 @@ int ln_tpr(int N) {
 int ln_parts(long M, int N) {
   if (N > LN_WIDE) return (int)std::min<long>(std::max<long>(M, 1), 64);
   const int tpr = ln_tpr(N), rpb = std::max(256, tpr) / tpr;
+  // up to eight rows in turn, one launch: 64 x 256 takes 12.1 us a call in a loop and 27.9 alone; a row at a time and a join
+  // 15.4 and 26.1
+  if (tpr <= 64 && M <= 8L * rpb) return 1;
   return (int)std::min<long>(std::max<long>(1, (M + rpb - 1) / rpb), tpr > 256 ? 512 : 1024);
 }
 
