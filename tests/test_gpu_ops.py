@@ -346,6 +346,20 @@ def test_diff_attention_autograd_matches_bwd():
     assert all(torch.equal(a.grad, b) for a, b in zip(leaves, ref))
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_diff_attention_short_rows_keep_their_precision(dt):
+    """Two roundings reach dQ and dK, of dS and of the result, of one relative size and independent: sqrt(2) of the result's own
+    rounding in the norm.  A third, of the row sums, would make it sqrt(3); 1.5 stands between (1.41 < 1.5 < 1.73)."""
+    import tossctr
+    q, k, v, lam, do = da_inputs(gen(57), 7, 17, 17, 4, 2, 128, dt)
+    ref = da_ref(q, k, v, lam, do, True, 128 ** -0.5, None, None)
+    out, saved = tossctr.diff_attention_fwd(q, k, v, lam, causal=True)
+    dq, dk, _, _ = tossctr.diff_attention_bwd(do, q, k, v, lam, out, saved, causal=True)
+    for name, got in (("dq", dq), ("dk", dk)):
+        want = ref[name][0]
+        assert float((got.double() - want).norm()) <= 1.5 * float((want.to(dt).double() - want).norm()), name
+
+
 def test_diff_attention_gradient_of_a_sum():
     """The gradient that arrives is one element for all places (strides of 0)."""
     import tossctr

@@ -20,7 +20,7 @@
 // Roundings to 16 bits.  The forward's P enter the product with V as two 16-bit terms each (the value and what that leaves
 // out): O is a difference, and where the maps agree one rounding of either would be larger than the result's own.  In
 // the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.  What
-// the rounding of O left out is kept too: delta_1, taken from the rounded O alone, would add as much again to dQ of short rows.
+// the roundings of O and of P_2 V left out is kept too: deltas from the rounded ones would add as much again to dQ of short rows.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,7 +33,8 @@ namespace {
 struct DaArgs {
   const void *q, *k, *v, *dout;
   const float* lam;
-  void *o, *o2, *ol;             // (B, T, H, 2 D); kept for the backward (may be null): o2 = P_2 V, ol = what o's rounding left out
+  void *o, *o2, *ol;             // (B, T, H, 2 D); kept for the backward (may be null): o2 = P_2 V and, `plane` elements
+                                 // on, what its rounding left out; ol = what o's rounding left out
   float* stat;                   // 2 planes of rows: log2 sums of the maps
   void *dq, *dk, *dv;
   float* dlam;
@@ -41,7 +42,7 @@ struct DaArgs {
   float* kvpart;                 // backward, split rows: partial dK, dV
   const int *q_lens, *kv_lens;
   long q_sb, q_st, q_sh, q_sc, k_sb, k_ss, k_sh, k_sc, v_sb, v_ss, v_sh, g_sb, g_st, g_sh;
-  long rows;                     // B Hkv R
+  long rows, plane;              // B Hkv R; B T H 2 D
   float c, scale;                // scale log2(e), scale
   int B, T, S, H, Hkv, G, R, causal, splits, tiles, tiles32;
 };
@@ -368,6 +369,9 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = none ? 0.f : o[j][4 * r4 + r] * inv;
         put((T*)a.o2 + at, j, r4, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] -= (float)(T)x[r];
+        put((T*)a.o2 + a.plane + at, j, r4, x);
       }
   } else {
     const float lam = a.lam[head];
@@ -446,6 +450,7 @@ __global__ __launch_bounds__(32 * GR) void da_join(const DaArgs a) {
   ((T*)a.o)[out] = (T)u;
   if (a.o2) {
     ((T*)a.o2)[out] = (T)w;
+    ((T*)a.o2)[a.plane + out] = (T)(w - (float)(T)w);
     ((T*)a.ol)[out] = (T)(u - (float)(T)u);
   }
   if (a.stat && blockIdx.y == 0 && col < 2) {
@@ -521,11 +526,12 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
   for (int k = 0; k < KV; ++k) {
     gf[k] = *(const v8*)(gp + 16 * k + 8 * h);
     const long at = orow + 16 * k + 8 * h;
-    const v8 o = *(const v8*)((const T*)a.o + at), o2 = *(const v8*)((const T*)a.o2 + at), ol = *(const v8*)((const T*)a.ol + at);
+    const v8 o = *(const v8*)((const T*)a.o + at), o2 = *(const v8*)((const T*)a.o2 + at), ol = *(const v8*)((const T*)a.ol + at),
+             o2l = *(const v8*)((const T*)a.o2 + a.plane + at);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       d1 = fmaf((float)gf[k][i], (float)o[i] + (float)ol[i], d1);
-      d2 = fmaf((float)gf[k][i], (float)o2[i], d2);
+      d2 = fmaf((float)gf[k][i], (float)o2[i] + (float)o2l[i], d2);
     }
   }
   d1 += __shfl_xor(d1, 32, 64);
@@ -936,6 +942,7 @@ DaArgs da_args(const ctr_diffattn_t* p) {
   a.c = p->scale * 1.44269504088896341f;
   a.B = p->B; a.T = p->T; a.S = p->S; a.H = p->H; a.Hkv = p->Hkv; a.G = p->H / p->Hkv; a.R = p->T * a.G;
   a.rows = (long)p->B * p->Hkv * a.R;
+  a.plane = a.rows * 2 * p->D;
   a.causal = p->causal;
   a.splits = 1;
   return a;

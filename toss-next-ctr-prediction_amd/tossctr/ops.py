@@ -224,9 +224,9 @@ def diff_attention_fwd(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_l
     saved = None
     a.o = out.data_ptr()
     if save:
-        parts = q.new_empty((2, a.B, a.T, a.H, 2 * a.D))     # the second map's, out's remainder
+        parts = q.new_empty((3, a.B, a.T, a.H, 2 * a.D))     # the second map's and its remainder, out's remainder
         stat = q.new_empty((2, a.B * a.H * a.T), dtype=torch.float32)
-        a.o2, a.ol, a.stat = parts.data_ptr(), parts.data_ptr() + 2 * out.numel(), stat.data_ptr()
+        a.o2, a.ol, a.stat = parts.data_ptr(), parts.data_ptr() + 4 * out.numel(), stat.data_ptr()
         saved = (parts, stat)
     if out.numel():
         ref = C.byref(a)
@@ -246,14 +246,14 @@ def diff_attention_bwd(dout, q, k, v, lam, out, saved, causal=False, scale=None,
     for t, what in ((dout, "dout"), (out, "out")):
         if tuple(t.shape) != shape or t.dtype != q.dtype:
             raise ValueError(f"diff_attention_bwd: {what} of shape {shape} {q.dtype}, got {tuple(t.shape)} {t.dtype}")
-    if tuple(parts.shape) != (2, *shape) or parts.dtype != q.dtype or not parts.is_contiguous() or \
+    if tuple(parts.shape) != (3, *shape) or parts.dtype != q.dtype or not parts.is_contiguous() or \
             tuple(stat.shape) != (2, a.B * a.H * a.T) or stat.dtype != torch.float32 or not stat.is_contiguous():
         raise ValueError("diff_attention_bwd: saved as diff_attention_fwd gave it")
     _device("diff_attention_bwd", q, dout, out, parts, stat)
     (dout, gs), (out, _) = _aligned(dout), _aligned(out.contiguous())
     dq, dk, dv, dlam = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape), lam.new_empty(a.H)
     a.o, a.stat = out.data_ptr(), stat.data_ptr()
-    a.o2, a.ol = parts.data_ptr(), parts.data_ptr() + 2 * out.numel()
+    a.o2, a.ol = parts.data_ptr(), parts.data_ptr() + 4 * out.numel()
     ref = C.byref(a)
     size = query("ctr_diffattn_bwd_ws_size", ref)
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
