@@ -1,0 +1,56 @@
+"""Differential attention over the range of float16 (tossctr.ops): probabilities far below a row's largest.  Against the definition
+in 64 bits, with bounds from the roundings."""
+import os
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from test_gpu_ops import BF, HF, U, gen, hold, randn  # noqa: E402
+
+
+# ---------------------------------------------------------------------------------------------- forward
+def fwd_ref(q, k, v, lam, scale):
+    """The output in 64 bits (no mask) and its bound: the result's own rounding u |O|; of P the two 16-bit terms leave u^2 of it,
+    in float16 at least 2^-39 of the row's largest; and the fp32 steps under it -- 2 D roundings of a score's absolute sum and
+    three of its value, through the exponential, and 2 S + 8 of sums, quotient and difference."""
+    u, (B, T, H, _, D), S = U[q.dtype], q.shape, k.shape[1]
+    G = H // k.shape[2]
+    qq = q.double().permute(3, 0, 2, 1, 4)                                    # 2 B H T D
+    kk = k.double().repeat_interleave(G, 2).permute(3, 0, 2, 1, 4)            # 2 B H S D
+    vv = v.double().repeat_interleave(G, 2).transpose(1, 2)                   # B H S DV
+    s = qq @ kk.transpose(-1, -2) * scale
+    p = s.softmax(-1)
+    lm = lam.double()[None, :, None, None]
+    out = (p[0] - lm * p[1]) @ vv
+    size = float((qq.abs() @ kk.abs().transpose(-1, -2)).max()) * scale
+    eps = 2.0 ** -23 * (1.4427 * (D * size + 3 * float(s.abs().max())) + 2 * S + 8)
+    pv = (p[0] + lm.abs() * p[1]) @ vv.abs()
+    least = 2.0 ** -39 * (1 + lm.abs()) * vv.abs().sum(-2, keepdim=True) if q.dtype == HF else 0.0
+    bound = u * out.abs() + (u * u + eps) * pv + least
+    return out.transpose(1, 2), bound.transpose(1, 2)
+
+
+@pytest.mark.parametrize("nats", [5.0, 12.0, 15.0, 17.0, 17.5, 19.0])
+@pytest.mark.parametrize("dt,D,S,B", [(HF, 64, 4097, 3), (BF, 64, 4097, 3), (HF, 128, 700, 1), (HF, 32, 9000, 1)])
+def test_one_key_far_above_the_others(dt, D, S, B, nats):
+    """A first key that takes nearly all of every row and has no value, the others `nats` below it with values of one sign: what
+    they give together is the output.  (9000 keys and one batch: the keys are split.)"""
+    import tossctr
+    g = gen(int(10 * nats) + S)
+    T, H = 45, 2
+    q, k = torch.zeros(B, T, H, 2, D, device="cuda"), torch.zeros(B, S, H, 2, D, device="cuda")
+    q[..., 0] = 1.0
+    k[:, 0, :, :, 0] = nats
+    k[:, 1:, :, :, 1:] = 0.05 * randn(g, B, S - 1, H, 2, D - 1)       # the queries are 0 there but for a little
+    q[..., 1:] = 0.05 * randn(g, B, T, H, 2, D - 1)
+    v = 1 + 0.5 * torch.rand(B, S, H, 2 * D, device="cuda", generator=g)
+    v[:, 0] = 0.0
+    lam = torch.tensor([0.5, -0.25], device="cuda")
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    for t in (T, 1):
+        out, _ = tossctr.diff_attention_fwd(q[:, :t], k, v, lam, scale=1.0, save=False)
+        hold(f"out {t}", out, *fwd_ref(q[:, :t], k, v, lam, 1.0), dt)

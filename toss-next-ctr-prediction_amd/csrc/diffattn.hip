@@ -15,10 +15,12 @@
 // tile's products, one barrier a tile; rows behind the end are out of the load's range and come as zeros.  A tile is
 // read once along a row (ds_read_b128) and once down the columns (the LDS transpose read); the 16-byte chunks of a row
 // are XORed with the row, in the global address, so that both reads are free of bank conflicts.
-// Softmax in base 2 with one running maximum per map, taken up only when a score passes it by 2^8; statistics,
+// Softmax in base 2 with one running maximum per map, taken up only when a score passes it by 2^8 (fp16: 2); statistics,
 // accumulators and dlam's sum are fp32.
 // Roundings to 16 bits.  The forward's P enter the product with V as two 16-bit terms each (the value and what that leaves
-// out): O is a difference, and where the maps agree one rounding of either would be larger than the result's own.  In
+// out): O is a difference, and where the maps agree one rounding of either would be larger than the result's own.  fp16's are
+// scaled up by 2^14, so that a probability keeps both terms down to 2^-17 of its row's largest, one down to 2^-28, and is held to
+// 2^-39 of it below (unscaled, many keys 15 nats below one of no value lost 3 % of the output, at 17.5 nats all of it).  In
 // the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.  What
 // the roundings of O and of P_2 V left out is kept too: deltas from the rounded ones would add as much again to dQ of short rows.
 #include <algorithm>
@@ -62,6 +64,12 @@ template <> struct Mfma<_Float16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
 };
+
+// The forward's exponentials are 2^(UP + s - m) with m at most LAG bits below the largest score: fp16 takes them as near to the top
+// of its range as they go (2^15), bf16 has fp32's range.  The factor cancels in the quotient and in the joins.  The smaller LAG takes
+// the maximum up more often: 1531 rows on 5627 keys, fp16, D = 128, 314 us unscaled (LAG 8), 317 at 11 + 4, 321 at 13 + 2, 326 so.
+template <typename T> struct Prob { static constexpr float UP = 0.f, LAG = 8.f; };
+template <> struct Prob<_Float16> { static constexpr float UP = 14.f, LAG = 1.f; };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -229,7 +237,7 @@ struct Seq {
 // under another's products.  RG pairs a workgroup.  Two 16-bit terms of P make 20 D operations a pair of the 12 D that the
 // definition has; the exponentials and their packing take as long as the products and hide only in part.  Measured: causal
 // 2 x 4096, 16 over 4 heads, D = 64, bf16: 336 us, 0.22 PFLOP/s of the definition's, 0.37 issued; 1531 rows on 5627 keys, 16
-// over 8 heads, D = 128, fp16: 333 us, 0.55 and 0.92 PFLOP/s.  One token on 131072 keys, 8 over 2 heads, D = 128: 42 us, 6.4 TB/s.
+// over 8 heads, D = 128, fp16: 326 us, 0.56 and 0.93 PFLOP/s.  One token on 131072 keys, 8 over 2 heads, D = 128: 42 us, 6.4 TB/s.
 // Workgroups: (batch, key head) fastest, so that the eight XCDs, which take workgroups in turn, each keep few heads'
 // keys in their L2; then the splits, then the row tiles, the causally longest first.
 template <typename T, int D, int RG>
@@ -286,14 +294,14 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, sc[r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any((top - m) * a.c > 8.f)) {        // also the first keys, from -inf (-inf - -inf is NaN: no)
+    if (__any((top - m) * a.c > Prob<T>::LAG)) {        // also the first keys, from -inf (-inf - -inf is NaN: no)
       const float mn = fmaxf(m, top), f = m == mn ? 1.f : exp2f((m - mn) * a.c);
       l *= f;
 #pragma unroll
       for (int j = 0; j < NO; ++j) o[j] *= f;
       m = mn;
     }
-    const float base = m == -INFINITY ? 0.f : m * a.c;
+    const float base = m == -INFINITY ? 0.f : fmaf(m, a.c, -Prob<T>::UP);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], a.c, -base));
@@ -342,7 +350,7 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
   const bool none = l == 0.f;                  // sees no key: zeros, whatever the keys' values are
   const float inv = none ? 0.f : 1.f / l;
   if (a.stat && h == 0 && row < a.R)           // a row that sees nothing: +inf, so that its P comes out 0
-    a.stat[map * a.rows + n] = none ? INFINITY : fmaf(m, a.c, log2f(l));
+    a.stat[map * a.rows + n] = none ? INFINITY : fmaf(m, a.c, log2f(l) - Prob<T>::UP);
   // the second map's part goes through LDS to the first map's wave (each path by itself: a value that both change would be
   // copied register by register)
   float* meet = (float*)&tiles[0][0] + pair * DV * 32 + (lane & 31);
@@ -455,7 +463,7 @@ __global__ __launch_bounds__(32 * GR) void da_join(const DaArgs a) {
   }
   if (a.stat && blockIdx.y == 0 && col < 2) {
     const float ll = col ? l[1] : l[0], mm = col ? m[1] : m[0];
-    a.stat[col * a.rows + n] = ll == 0.f ? INFINITY : fmaf(mm, a.c, log2f(ll));
+    a.stat[col * a.rows + n] = ll == 0.f ? INFINITY : fmaf(mm, a.c, log2f(ll) - Prob<T>::UP);
   }
 }
 
