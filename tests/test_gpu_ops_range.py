@@ -1,5 +1,6 @@
-"""Differential attention over the range of float16 (tossctr.ops): probabilities far below a row's largest.  Against the definition
-in 64 bits, with bounds from the roundings."""
+"""Differential attention over the range of float16 (tossctr.ops): probabilities far below a row's largest, gradients and rows of
+far sizes.  Against the definition in 64 bits, with bounds from the roundings."""
+import math
 import os
 import sys
 
@@ -9,7 +10,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_ops import BF, HF, U, gen, hold, randn  # noqa: E402
+from test_gpu_ops import BF, HF, U, da_inputs, da_ref, gen, hold, randn  # noqa: E402
 
 
 # ---------------------------------------------------------------------------------------------- forward
@@ -54,3 +55,42 @@ def test_one_key_far_above_the_others(dt, D, S, B, nats):
     for t in (T, 1):
         out, _ = tossctr.diff_attention_fwd(q[:, :t], k, v, lam, scale=1.0, save=False)
         hold(f"out {t}", out, *fwd_ref(q[:, :t], k, v, lam, 1.0), dt)
+
+
+# ---------------------------------------------------------------------------------------------- backward
+def test_float16_rows_of_far_sizes():
+    """Rows of a tile whose dS lie 2^34 apart, over keys of sizes that bring their dQ into float16's range: each keeps its bits."""
+    import tossctr
+    q, k, v, lam, do = da_inputs(gen(3), 2, 64, 50, 2, 2, 64, HF)
+    q = (q * 2.0 ** -8).to(HF)
+    q[:, ::2, ..., 0], q[:, 1::2, ..., 0] = 8.0, -8.0          # even rows see the first keys, odd ones the others
+    k[:, :25] *= 2.0 ** -6
+    k[:, 25:] *= 2.0 ** 5
+    k[:, :25, ..., 0], k[:, 25:, ..., 0] = 8.0, -8.0
+    do = do.clamp(-3, 3)
+    do[:, ::2] *= 2.0 ** 14
+    do[:, 1::2] = torch.sign(do[:, 1::2]) * 2.0 ** -20
+    ref = da_ref(q, k, v, lam, do, False, 1.0, None, None)
+    out, saved = tossctr.diff_attention_fwd(q, k, v, lam, scale=1.0)
+    grads = tossctr.diff_attention_bwd(do, q, k, v, lam, out, saved, scale=1.0)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        want, bound = ref[name]
+        far = want.abs() >= 65520          # float16 rounds these to infinity (some of dK: 32 rows of 2^13 times 8)
+        assert name == "dk" or not far.any()
+        assert torch.equal(got[far].double(), torch.sign(want[far]) * math.inf)
+        hold(name, got.masked_fill(far, 0.0), want.masked_fill(far, 0.0), bound.masked_fill(far, 0.0), HF)
+
+
+def test_an_infinite_row_stays_alone():
+    """A row whose gradient holds an infinity leaves the other rows' dQ as they are without it."""
+    import tossctr
+    for dt in (HF, BF):
+        q, k, v, lam, do = da_inputs(gen(9), 1, 40, 70, 2, 1, 64, dt)
+        got = []
+        for x in (0.0, math.inf):
+            do[:, 7] = 0.0
+            do[:, 7, :, 3] = x
+            out, saved = tossctr.diff_attention_fwd(q, k, v, lam)
+            got.append(tossctr.diff_attention_bwd(do, q, k, v, lam, out, saved)[0])
+        others = torch.arange(40, device="cuda") != 7
+        assert torch.equal(got[0][:, others], got[1][:, others]), dt

@@ -21,7 +21,8 @@
 // out): O is a difference, and where the maps agree one rounding of either would be larger than the result's own.  fp16's are
 // scaled up by 2^14, so that a probability keeps both terms down to 2^-17 of its row's largest, one down to 2^-28, and is held to
 // 2^-39 of it below (unscaled, many keys 15 nats below one of no value lost 3 % of the output, at 17.5 nats all of it).  In
-// the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows its size.  What
+// the backward P_1 - lam P_2 and dS are rounded once; fp16's dS is first scaled by a power of two that follows
+// its size, a row's own in dQ and a key's own in dK.  What
 // the roundings of O and of P_2 V left out is kept too: deltas from the rounded ones would add as much again to dQ of short rows.
 #include <algorithm>
 #include <type_traits>
@@ -468,22 +469,20 @@ __global__ __launch_bounds__(32 * GR) void da_join(const DaArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// Power-of-two scale under which a tile of dS fits fp16 with all its bits: it starts beyond every value and comes down,
-// with the accumulators, when a tile would pass 2^15 (bf16 has fp32's range: always 1)
+// Power-of-two scale under which a column (a row of dQ, a key of dK) fits fp16 with all its bits: it starts beyond every value and
+// comes down, with the column's accumulators, when one would pass 2^15; values down to 2^-29 of the column's largest keep 11 bits.
+// A lane's own: under one scale for the tile a column far below its neighbours lost its bits, and an infinity in one reached all.
+// (bf16 has fp32's range: always 1)
 template <typename T>
-struct DsScale {
+struct ColScale {
   static constexpr bool ON = __is_same(T, _Float16);
   float f;
-  __device__ __forceinline__ DsScale() : f(ON ? 0x1p100f : 1.f) {}
-  // returns the accumulators' factor (1: nothing to do)
-  __device__ __forceinline__ float fit(const f32x16& x, const f32x16& y) {
-    if constexpr (!ON) return 1.f;
-    float top = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(fabsf(x[r]), fabsf(y[r])));
-    if (!__any(top * f > 32768.f)) return 1.f;
-    top = wave_max(top);
-    if (!(top < 0x1p120f)) return 1.f;         // infinities and NaN stay what they are
+  __device__ __forceinline__ ColScale() : f(ON ? 0x1p100f : 1.f) {}
+  // top: the largest size among the lane's values; returns the accumulators' factor (1: nothing to do).  All lanes take part.
+  __device__ __forceinline__ float fit(float top) {
+    if (!ON || !__any(top * f > 32768.f)) return 1.f;
+    top = fmaxf(top, __shfl_xor(top, 32, 64));           // the column's other half
+    if (!(top * f > 32768.f) || !(top < INFINITY)) return 1.f;      // infinities and NaN stay what they are
     int e;
     frexpf(top, &e);
     const float nf = ldexpf(1.f, 12 - e), down = nf / f;
@@ -491,6 +490,14 @@ struct DsScale {
     return down;
   }
 };
+template <typename T>
+__device__ __forceinline__ float top_of(const f32x16& x, float top = 0.f) {
+  if constexpr (ColScale<T>::ON) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+  }
+  return top;
+}
 
 // acc[j] += (columns 32 j .. of a panel of width W)^T x
 template <typename T, int W, int N>
@@ -553,7 +560,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
 #pragma unroll
     for (int j = 0; j < NQ; ++j) dq[c][j] = 0.f;
   float dl = 0.f;
-  DsScale<T> fit;
+  ColScale<T> fit;
   const uint32_t kcol = col_base<T, D>(tiles[0], lane);
   int cur = 0;
   for (int kb = 0; kb < k1; kb += 32, cur ^= 1) {
@@ -592,14 +599,14 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
 #pragma unroll
     for (int r = 0; r < 16; ++r) dl_tile += dp[r];
     dl += dl_tile;
-    const float down = fit.fit(sc[0], sc[1]);
-    if (down != 1.f) {
+    const float down = fit.fit(top_of<T>(sc[1], top_of<T>(sc[0])));
+    if (__any(down != 1.f)) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) dq[c][j] *= down;
     }
-    if constexpr (DsScale<T>::ON) {
+    if constexpr (ColScale<T>::ON) {
       sc[0] *= fit.f;
       sc[1] *= fit.f;
     }
@@ -668,7 +675,7 @@ __global__ __launch_bounds__(1024) void da_dlam(const DaArgs a) { head_dlam(a, b
 template <typename T, int D, int NP>
 __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const DaArgs a) {
   constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32, NW = 2 * NP, TILE = Stage<T, D, NW>::TILE;
-  constexpr bool HALF = DsScale<T>::ON;
+  constexpr bool HALF = ColScale<T>::ON;
   constexpr float PS = HALF ? 1024.f : 1.f;       // |P_1 - lam P_2| <= max(1, |lam|): keeps fp16's P out of the subnormals
   typedef Stage<T, D, NW> St;
   typedef typename Vec<T>::v8 v8;
@@ -809,7 +816,7 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
     f32x16 dk[2][NQ];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) dk[0][j] = dk[1][j] = 0.f;
-    DsScale<T> fit;
+    ColScale<T> fit;
     const uint32_t qcol = col_base<T, D>(tiles[0], lane);
     int cur = 0;
     for (int rb = r0; rb < r1; rb += 32, cur ^= 1) {
@@ -841,8 +848,8 @@ __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const Da
           ds[1][r] = p2[j] * fmaf(-lam[j], dp[r], d2[j]);
         }
       }
-      const float down = fit.fit(ds[0], ds[1]);
-      if (down != 1.f) {
+      const float down = fit.fit(top_of<T>(ds[1], top_of<T>(ds[0])));
+      if (__any(down != 1.f)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
