@@ -1,5 +1,5 @@
 """Differential attention over the range of float16 (tossctr.ops): probabilities far below a row's largest, gradients and rows of
-far sizes.  Against the definition in 64 bits, with bounds from the roundings."""
+far sizes, weights of any size.  Against the definition in 64 bits, with bounds from the roundings."""
 import math
 import os
 import sys
@@ -10,7 +10,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_ops import BF, HF, U, da_inputs, da_ref, gen, hold, randn  # noqa: E402
+from test_gpu_ops import BF, HF, U, da_case, da_inputs, da_ref, gen, hold, randn  # noqa: E402
 
 
 # ---------------------------------------------------------------------------------------------- forward
@@ -58,6 +58,50 @@ def test_one_key_far_above_the_others(dt, D, S, B, nats):
 
 
 # ---------------------------------------------------------------------------------------------- backward
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("T,S", [(1, 1), (40, 40), (5, 300)])
+def test_lam_of_any_size(dt, T, S):
+    """Rows that see one key have P_1 = P_2 = 1, and P_1 - lam P_2 passes every 16-bit range that is not fitted to it."""
+    q, k, v, _, do = da_inputs(gen(T + S), 2, T, S, 6, 2, 32, dt)
+    lam = torch.tensor([70.0, -70.0, 1e3, -3e4, 1e-5, 0.0], device="cuda")
+    da_case(q, k, (v * 2.0 ** -10).to(dt), lam, (do * 2.0 ** -6).to(dt), causal=T == S)
+
+
+def floors(q, k, v, lam, do, scale):
+    """What float16 leaves of dS and P_1 - lam P_2 beside u of them (no mask, one key head): scaled so that a row's (in dQ) or a
+    key's (in dK, dV) largest stands at 2^11 or more, a value is held to half of the type's smallest step, 2^-25, which is 2^-36 of
+    that largest; it meets every key (query, dO)."""
+    qq, kk, vv, dd = (t.double().transpose(1, 2) for t in (q.flatten(3), k.flatten(3), v, do))       # B H T 2D, B 1 S 2D, ...
+    D, lm = q.shape[-1], lam.double()[None, :, None, None]
+    qs, ks = (qq[..., :D], qq[..., D:]), (kk[..., :D], kk[..., D:])
+    p = [(a @ b.transpose(-1, -2) * scale).softmax(-1) for a, b in zip(qs, ks)]
+    dp = dd @ vv.transpose(-1, -2)
+    ds = [x * (dp - (x * dp).sum(-1, keepdim=True)) for x in p]
+    row = 2.0 ** -36 * torch.maximum(ds[0].abs(), ds[1].abs()).amax(-1, keepdim=True)
+    dq = torch.cat([scale * row * w * b.abs().sum(-2, keepdim=True) for w, b in zip((1, lm.abs()), ks)], -1)
+    key = 2.0 ** -36 * torch.maximum(ds[0].abs(), (lm * ds[1]).abs()).amax((1, 2))[:, None, :, None]
+    dk = torch.cat([scale * key * a.abs().sum((1, 2), keepdim=True) for a in qs], -1)
+    dv = 2.0 ** -36 * (p[0] - lm * p[1]).abs().amax((1, 2))[:, None, :, None] * dd.abs().sum((1, 2), keepdim=True)
+    return {"dq": dq.transpose(1, 2).unflatten(-1, (2, D)), "dk": dk.transpose(1, 2).unflatten(-1, (2, D)), "dv": dv.transpose(1, 2)}
+
+
+@pytest.mark.parametrize("bits", [20, 26, 30])
+def test_float16_gradients_of_keys_far_below(bits):
+    """Keys whose probabilities are 2^-20 ... 2^-30 of their neighbours' in every row: their dK and dV keep their bits."""
+    import tossctr
+    q, k, v, lam, do = da_inputs(gen(bits), 1, 200, 64, 2, 1, 32, HF)
+    q, k = 0.1 * q.float(), 0.1 * k.float()
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    k[:, ::2, :, :, 0] = -bits * math.log(2)
+    q, k, do = q.to(HF), k.to(HF), do * 2.0 ** 10
+    ref, least = da_ref(q, k, v, lam, do, False, 1.0, None, None), floors(q, k, v, lam, do, 1.0)
+    out, saved = tossctr.diff_attention_fwd(q, k, v, lam, scale=1.0)
+    grads = tossctr.diff_attention_bwd(do, q, k, v, lam, out, saved, scale=1.0)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        hold(name, got, ref[name][0], ref[name][1] + least[name], HF)
+
+
 def test_float16_rows_of_far_sizes():
     """Rows of a tile whose dS lie 2^34 apart, over keys of sizes that bring their dQ into float16's range: each keeps its bits."""
     import tossctr
