@@ -685,10 +685,9 @@ int ctr_ln_bwd(const void* dy, long lddy, const void* x, long ldx, const float* 
  * head serves H / Hkv consecutive query heads).  o (B, T, H, 2 D) contiguous.  q_lens / kv_lens (B) nullable: valid
  * positions and keys of each sequence, held to [0, T] / [0, S]; what stands behind
  * kv_lens does not count.  causal: position t sees the keys up to t + kv_len - q_len.  A row that sees no key, and a position behind q_len, gives zeros (and zero
- * gradients).  For the backward pass o2 (2, B, T, H, 2 D: the
- * second map's part, then what its rounding left out), ol (B, T, H, 2 D: what o's rounding left out; both of o's type)
- * and stat (2 * B * H * T floats: the rows' log-sums) are written by the forward; all null:
- * inference.
+ * gradients).  For the backward pass o2 (2, B, T, H, 2 D: the second map's part, then what its rounding left out), ol (B, T, H,
+ * 2 D: what o's rounding left out; both of o's type, what was left out times 2^11 in fp16) and stat (2 * B * H * T floats: the
+ * rows' log-sums) are written by the forward; all null: inference.
  * ctr_diffattn_bwd: dout (B, T, H, 2 D) with strides; dq, dk, dv contiguous in the shapes of q, k, v; dlam (H) fp32.  */
 typedef struct {
   const void *q, *k, *v;

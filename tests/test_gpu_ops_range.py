@@ -138,3 +138,16 @@ def test_an_infinite_row_stays_alone():
             got.append(tossctr.diff_attention_bwd(do, q, k, v, lam, out, saved)[0])
         others = torch.arange(40, device="cuda") != 7
         assert torch.equal(got[0][:, others], got[1][:, others]), dt
+
+
+def test_float16_small_values_keep_the_row_sums():
+    """Values of a few of float16's smallest steps under gradients of thousands: the row sums of the backward come from outputs
+    that a 16-bit number, and what its rounding left out at the same scale, would not hold."""
+    g = gen(13)
+    q, k, v, lam, do = da_inputs(g, 2, 40, 60, 4, 2, 64, HF)
+    v = (v * 2.0 ** -21).to(HF)
+    do = (do * 2.0 ** 13).clamp(-6e4, 6e4).to(HF)
+    q, k = (q / 16).to(HF), (k * 16).to(HF)
+    ref = da_ref(q, k, v, lam, do, False, 1 / 8, None, None)
+    assert float(ref["dq"][0].abs().mean()) > 2.0 ** -12            # far above float16's smallest step
+    da_case(q, k, v, lam, do)

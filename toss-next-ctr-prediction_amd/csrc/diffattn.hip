@@ -24,6 +24,8 @@
 // the backward P_1 - lam P_2 and dS are rounded once, in fp16 under a power of two that follows their size, a row's own in dQ and
 // a key's own in dK and dV.  What
 // the roundings of O and of P_2 V left out is kept too: deltas from the rounded ones would add as much again to dQ of short rows.
+// delta_1 is of O + lam P_2 V, so its error grows with lam: |lam| 2^-17 (fp16 2^-23) of |dO| |P_2 V|, below dS's own rounding up to
+// |lam| of a few hundred.
 #include <algorithm>
 #include <type_traits>
 
@@ -37,7 +39,7 @@ struct DaArgs {
   const void *q, *k, *v, *dout;
   const float* lam;
   void *o, *o2, *ol;             // (B, T, H, 2 D); kept for the backward (may be null): o2 = P_2 V and, `plane` elements
-                                 // on, what its rounding left out; ol = what o's rounding left out
+                                 // on, what its rounding left out; ol = what o's rounding left out (rest())
   float* stat;                   // 2 planes of rows: log2 sums of the maps
   void *dq, *dk, *dv;
   float* dlam;
@@ -113,6 +115,11 @@ __device__ __forceinline__ typename Vec<T>::v8 frag_col(uint32_t base, int i, in
   const auto v = __builtin_bit_cast(typename Vec<T>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q));
   return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+// What the rounding of a kept output left out, x - T(x), in T again: fp16's is kept 2^11 times as large, since that of a value below
+// 2^-13 would fall under the type's smallest step.
+template <typename T> constexpr float REST = __is_same(T, _Float16) ? 2048.f : 1.f;
+template <typename T>
+__device__ __forceinline__ float rest(float x) { return (x - (float)(T)x) * REST<T>; }
 // registers 8 i .. 8 i + 7 of a C tile as an operand, and what the rounding left out
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::v8 pack(const f32x16& v, int i) {
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
         for (int r = 0; r < 4; ++r) x[r] = none ? 0.f : o[j][4 * r4 + r] * inv;
         put((T*)a.o2 + at, j, r4, x);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] -= (float)(T)x[r];
+        for (int r = 0; r < 4; ++r) x[r] = rest<T>(x[r]);
         put((T*)a.o2 + a.plane + at, j, r4, x);
       }
   } else {
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(128 * RG, D == 128 ? (RG == 2 ? 2 : 1) : 3) void da
         put((T*)a.o + at, j, r4, x);
         if (a.ol) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] -= (float)(T)x[r];
+          for (int r = 0; r < 4; ++r) x[r] = rest<T>(x[r]);
           put((T*)a.ol + at, j, r4, x);
         }
       }
@@ -459,8 +466,8 @@ __global__ __launch_bounds__(32 * GR) void da_join(const DaArgs a) {
   ((T*)a.o)[out] = (T)u;
   if (a.o2) {
     ((T*)a.o2)[out] = (T)w;
-    ((T*)a.o2)[a.plane + out] = (T)(w - (float)(T)w);
-    ((T*)a.ol)[out] = (T)(u - (float)(T)u);
+    ((T*)a.o2)[a.plane + out] = (T)rest<T>(w);
+    ((T*)a.ol)[out] = (T)rest<T>(u);
   }
   if (a.stat && blockIdx.y == 0 && col < 2) {
     const float ll = col ? l[1] : l[0], mm = col ? m[1] : m[0];
@@ -547,8 +554,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaAr
              o2l = *(const v8*)((const T*)a.o2 + a.plane + at);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      d1 = fmaf((float)gf[k][i], (float)o[i] + (float)ol[i], d1);
-      d2 = fmaf((float)gf[k][i], (float)o2[i] + (float)o2l[i], d2);
+      d1 = fmaf((float)gf[k][i], fmaf((float)ol[i], 1.f / REST<T>, (float)o[i]), d1);
+      d2 = fmaf((float)gf[k][i], fmaf((float)o2l[i], 1.f / REST<T>, (float)o2[i]), d2);
     }
   }
   d1 += __shfl_xor(d1, 32, 64);
