@@ -1,5 +1,6 @@
-"""Differential attention over the range of float16 (tossctr.ops): probabilities far below a row's largest, gradients and rows of
-far sizes, weights of any size.  Against the definition in 64 bits, with bounds from the roundings."""
+"""Differential attention and Newton-Schulz over the range of their types (tossctr.ops): probabilities far below a row's largest,
+gradients and rows of far sizes, weights of any size, structured matrices.  Against the definitions in 64 bits, with bounds from
+the roundings."""
 import math
 import os
 import sys
@@ -10,7 +11,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_gpu_ops import BF, HF, U, da_case, da_inputs, da_ref, gen, hold, randn  # noqa: E402
+from test_gpu_ops import BF, F32, HF, NS_TOL, U, da_case, da_inputs, da_ref, gen, hold, ns_ref, randn, rel  # noqa: E402
 
 
 # ---------------------------------------------------------------------------------------------- forward
@@ -151,3 +152,35 @@ def test_float16_small_values_keep_the_row_sums():
     ref = da_ref(q, k, v, lam, do, False, 1 / 8, None, None)
     assert float(ref["dq"][0].abs().mean()) > 2.0 ** -12            # far above float16's smallest step
     da_case(q, k, v, lam, do)
+
+
+# ---------------------------------------------------------------------------------------------- Newton-Schulz
+def structured(kind, m, n):
+    g = gen(m + n)
+    if kind == "signs":
+        return torch.sign(randn(g, m, 1)) * torch.sign(randn(g, 1, n))
+    if kind == "ones":
+        return torch.ones(m, n, device="cuda")
+    if kind == "thirds":
+        return torch.full((m, n), 1 / 3, device="cuda")
+    return randn(g, m, 3) @ randn(g, 3, n)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("kind", ["signs", "ones", "thirds", "rank 3"])
+def test_newton_schulz_structured_matrices(kind, dt):
+    """Matrices whose roundings do not average out, in every form (one workgroup, small and large tiles)."""
+    import tossctr
+    mats = [structured(kind, m, n).to(dt) for m, n in ((60, 90), (150, 333), (333, 150), (150, 500), (800, 1000))]
+    for x, o in zip(mats, tossctr.newton_schulz(mats)):
+        assert rel(o, ns_ref(x)) <= U[dt] + NS_TOL, tuple(x.shape)
+
+
+@pytest.mark.parametrize("shape", [(96, 160), (150, 333), (800, 1000)])
+def test_newton_schulz_16_bit_results_are_the_rounded_fp32_ones(shape):
+    """Whatever the size, a 16-bit matrix is worked on as its fp32 copy is: the result is that one's rounding."""
+    import tossctr
+    for dt in (BF, HF):
+        x = (randn(gen(5), *shape) * 1e-2).to(dt)
+        got, want = tossctr.newton_schulz(x), tossctr.newton_schulz(x.float())
+        assert torch.equal(got, want.to(dt))

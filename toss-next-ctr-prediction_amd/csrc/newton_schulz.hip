@@ -8,7 +8,9 @@
 // a factor of two.  A product of two such values is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 with fp32
 // accumulation; the lo lo term is 2^-24 of it.  Three fp16 products cost 3/16 of one fp32 matrix instruction's time, so
 // this is fp32's accuracy at up to five times its rate.  16-bit accuracy would not do: the polynomial multiplies the error
-// of a small singular value by a (3.44) a step, 485 times in five.  The squares of the norm are summed in fp64, where no
+// of a small singular value by a (3.44) a step, 485 times in five.  Nor would the hi parts do for a bf16 result's last step (2048 x
+// 8192: 1815 us instead of 1942): roundings of matrices with structure do not average out, all ones of 150 x 333 came out 1.2 half
+// steps of bf16 off before their own rounding.  The squares of the norm are summed in fp64, where no
 // fp32 input overflows or vanishes.
 #include <algorithm>
 #include <atomic>
@@ -197,7 +199,7 @@ using NsMid = NsTile<4, 2, 2, 3>;          // 256 x 128
 using NsLarge = NsTile<2, 4, 2, 2>;        // 256 x 256
 template <bool NN, class S>
 __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float16* B, int ldb, int r0, int c0, int k0, int k1,
-                                        _Float16* lds, bool hi_only, typename S::Acc& acc) {
+                                        _Float16* lds, typename S::Acc& acc) {
   constexpr int NI = S::NI, NJ = S::NJ, NST = S::NST, NA = S::R / 64, NB = S::C / 64, LOADS = NA + NB, RPL = 256 / S::C;
   static_assert(S::R % 128 == 0 && (S::C == 128 || S::C == 256), "loads dealt to eight waves");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -265,7 +267,6 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float
   const auto multiply = [&](const Frags& f) {
 #pragma unroll
     for (int pr = 0; pr < 3; ++pr) {    // lo hi, hi lo, hi hi; the accumulators in turn
-      if (pr < 2 && hi_only) continue;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -306,7 +307,6 @@ __device__ __forceinline__ void ns_tile(const _Float16* A, int lda, const _Float
         }
 #pragma unroll
         for (int pr = 0; pr < 3; ++pr) {
-          if (pr < 2 && hi_only) continue;
 #pragma unroll
           for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -356,7 +356,7 @@ __host__ __device__ inline int tri_tiles(int mp) { return mp / S::R * (mp / S::R
 // partials of X X^T (square = false) or A A over a share of K, lower tiles; the workgroups of an XCD (every eighth) take the
 // same share, whose rows so stay in its L2
 template <class S>
-__global__ __launch_bounds__(512, 2) void ns_gram(const NsArgs p, int buf, bool square, bool hi_only) {
+__global__ __launch_bounds__(512, 2) void ns_gram(const NsArgs p, int buf, bool square) {
   extern __shared__ __align__(16) _Float16 lds[];
   const int i = ns_find(p, blockIdx.x);
   const NsMat& q = p.mat[i];
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(512, 2) void ns_gram(const NsArgs p, int buf, bool 
   const int steps = K / NS_BK, per = (steps + splits - 1) / splits;
   const _Float16* x = square ? (const _Float16*)(p.ws + q.off_a) : (const _Float16*)(p.ws + q.off_x) + (long)buf * 2 * q.mp * K;
   typename S::Acc acc;
-  ns_tile<false, S>(x, K, x, K, ti * S::R, tj * S::C, min(steps, sp * per) * NS_BK, min(steps, (sp + 1) * per) * NS_BK, lds, hi_only, acc);
+  ns_tile<false, S>(x, K, x, K, ti * S::R, tj * S::C, min(steps, sp * per) * NS_BK, min(steps, (sp + 1) * per) * NS_BK, lds, acc);
   float* out = (float*)(p.ws + q.off_p) + (long)sp * q.mp * q.mp;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC * 32 * S::NI, wc = wave % S::WC * 32 * S::NJ;
 #pragma unroll
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(256) void ns_join(const NsArgs p, bool square) {
 // X' = W X; the last step writes the result in its own type and orientation.  An XCD takes every eighth panel of columns, with
 // all row tiles of one together.
 template <class S>
-__global__ __launch_bounds__(512, 2) void ns_apply(const NsArgs p, int buf, int last, bool hi_only) {
+__global__ __launch_bounds__(512, 2) void ns_apply(const NsArgs p, int buf, int last) {
   extern __shared__ __align__(16) _Float16 lds[];
   constexpr int NI = S::NI, NJ = S::NJ;
   const int i = ns_find(p, blockIdx.x);
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(512, 2) void ns_apply(const NsArgs p, int buf, int 
   const _Float16* x = (const _Float16*)(p.ws + q.off_x) + (long)buf * 2 * q.mp * q.np;
   _Float16* y = (_Float16*)(p.ws + q.off_x) + (long)(buf ^ 1) * 2 * q.mp * q.np;
   typename S::Acc acc;
-  ns_tile<true, S>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, hi_only, acc);
+  ns_tile<true, S>(W, q.mp, x, q.np, r0, c0, 0, q.mp, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / S::WC * 32 * NI, wc = wave % S::WC * 32 * NJ;
   const bool tall = q.rows > q.cols;
   if (last) {
@@ -865,21 +865,18 @@ extern "C" int ctr_newton_schulz(const ctr_ns_mat_t* mats, int count, int steps,
     const int ni = prefix([](const NsMat& q) { return q.mp / 64 * (q.np / 64); });
     ns_init<<<ni, 256, 0, s>>>(g);
     for (int k = 0; k < steps; ++k) {
-      // nothing multiplies the last step's error: a bf16 result (half a step 2^-8) takes its products from the hi parts alone,
-      // whose roundings, 2^-12 of each operand, add a twentieth to the result's own error
-      const bool hi_only = k + 1 == steps && steps > 1 && type == TY_BF16;
       for (int square = 0; square < 2; ++square) {
         const int ng = prefix([&](const NsMat& q) { return cdiv(square ? q.asplits : q.splits, 8) * 8 * (w ? tri_tiles<NsMid>(q.mp) : tri_tiles<NsSmall>(q.mp)); });
-        if (w) ns_gram<NsMid><<<ng, 512, NsMid::LDS, s>>>(g, k & 1, square, hi_only);
-        else ns_gram<NsSmall><<<ng, 512, NsSmall::LDS, s>>>(g, k & 1, square, hi_only);
+        if (w) ns_gram<NsMid><<<ng, 512, NsMid::LDS, s>>>(g, k & 1, square);
+        else ns_gram<NsSmall><<<ng, 512, NsSmall::LDS, s>>>(g, k & 1, square);
         const int nj = prefix([](const NsMat& q) { return (q.mp / 32) * (q.mp / 32 + 1) / 2; });
         ns_join<<<nj, 256, 0, s>>>(g, square);
       }
       const int tr = w ? 256 : 128, tc = w == 2 ? 256 : 128;
       const int na = prefix([&](const NsMat& q) { return q.mp / tr * (cdiv(q.np / tc, 8) * 8); });
-      if (w == 2) ns_apply<NsLarge><<<na, 512, NsLarge::LDS, s>>>(g, k & 1, k + 1 == steps, hi_only);
-      else if (w) ns_apply<NsMid><<<na, 512, NsMid::LDS, s>>>(g, k & 1, k + 1 == steps, hi_only);
-      else ns_apply<NsSmall><<<na, 512, NsSmall::LDS, s>>>(g, k & 1, k + 1 == steps, hi_only);
+      if (w == 2) ns_apply<NsLarge><<<na, 512, NsLarge::LDS, s>>>(g, k & 1, k + 1 == steps);
+      else if (w) ns_apply<NsMid><<<na, 512, NsMid::LDS, s>>>(g, k & 1, k + 1 == steps);
+      else ns_apply<NsSmall><<<na, 512, NsSmall::LDS, s>>>(g, k & 1, k + 1 == steps);
     }
     g.count = 0;
     off[w] = 0;
