@@ -178,10 +178,13 @@ struct Stage {
 
 // 64 lanes x 16 bytes from r at off to consecutive LDS places.  Nothing comes back in registers, and tile_ready() waits: as a
 // builtin it would have the compiler wait for it before any transpose read, whose address it does not see.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"      // m0 is a reserved register; it is named because it changes
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, const void* lds, uint32_t off) {
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t open_range(const void* p) { return buf_rsrc(p, 0x7ffffff0u); }
 
 // every wave's loads of the next tile are in LDS and every wave is done with the last one

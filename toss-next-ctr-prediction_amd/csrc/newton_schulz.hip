@@ -166,9 +166,12 @@ __global__ __launch_bounds__(256) void ns_init(const NsArgs p) {
 }
 
 // 64 lanes x 16 bytes to consecutive LDS places.  Nothing comes back in registers and the K loop waits for it by count.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"      // m0 is a reserved register; it is named because it changes
 __device__ __forceinline__ void ns_dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t off, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void ns_wait() {      // all but the last N loads have landed, in every wave
   static_assert(N <= 63, "vmcnt");
