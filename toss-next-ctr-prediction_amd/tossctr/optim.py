@@ -12,6 +12,7 @@ ever written.
 from __future__ import annotations
 
 import math
+import warnings
 
 import numpy as np
 import torch
@@ -615,8 +616,12 @@ class FusedMuon(FusedAdamW):
 
 
 def build_optimizer(model, cfg, ema=None, process_group=None):
-    """The optimizer that ``train.optimizer`` names: "muon" is FusedMuon, anything else the reference's AdamW."""
+    """The optimizer that ``train.optimizer`` names: "muon" is FusedMuon, "adamw" (or nothing) the reference's AdamW.  The reference
+    reads no name and takes AdamW for any (src/train.py:138), so another name is AdamW too, with a warning."""
     tr = cfg["train"]
-    cls = FusedMuon if str(tr.get("optimizer", "adamw")).lower() == "muon" else FusedAdamW
+    name = str(tr.get("optimizer") or "adamw").lower()
+    if name not in ("adamw", "muon"):
+        warnings.warn(f"train.optimizer {tr['optimizer']!r} is neither 'adamw' nor 'muon': AdamW is taken", stacklevel=2)
+    cls = FusedMuon if name == "muon" else FusedAdamW
     return cls(model, lr=tr["lr"], weight_decay=tr["weight_decay"], max_grad_norm=tr.get("grad_clip_norm", 0.0), ema=ema,
                process_group=process_group)
