@@ -1,6 +1,6 @@
 """Differential attention and Newton-Schulz over the range of their types (tossctr.ops): probabilities far below a row's largest,
-gradients and rows of far sizes, weights of any size, structured matrices.  Against the definitions in 64 bits, with bounds from
-the roundings."""
+gradients and rows of far sizes, weights of any size, structured matrices, lengths together with split keys and split rows.  Against
+the definitions in 64 bits, with bounds from the roundings."""
 import math
 import os
 import sys
@@ -56,6 +56,31 @@ def test_one_key_far_above_the_others(dt, D, S, B, nats):
     for t in (T, 1):
         out, _ = tossctr.diff_attention_fwd(q[:, :t], k, v, lam, scale=1.0, save=False)
         hold(f"out {t}", out, *fwd_ref(q[:, :t], k, v, lam, 1.0), dt)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("T,S,H,Hkv,D", [(1, 2, 4, 4, 32), (17, 3, 4, 2, 32), (40, 9, 2, 2, 64), (33, 33, 2, 1, 128)])
+def test_maps_that_nearly_agree(dt, T, S, H, Hkv, D):
+    """The second map's queries differ from the first's by a rounding or two and lam is 1: the difference is far smaller than
+    either product, and is held to what two 16-bit terms of P leave (one term leaves up to 2^7 (bf16) times the bound)."""
+    import tossctr
+    g = gen(T + S)
+    q, k, v, _, _ = da_inputs(g, 5, T, S, H, Hkv, D, dt)
+    q, k = (q * 0.5).to(dt), (k * 0.5).to(dt)
+    q[:, :, :, 1] = (q[:, :, :, 0].float() * (1 + 4 * U[dt] * randn(g, *q.shape[:3], D))).to(dt)
+    k[:, :, :, 1] = k[:, :, :, 0]
+    lam = torch.ones(H, device="cuda")
+    out, _ = tossctr.diff_attention_fwd(q, k, v, lam, save=False)
+    hold("out", out, *fwd_ref(q, k, v, lam, D ** -0.5), dt)
+
+
+@pytest.mark.parametrize("D,T,S", [(64, 90, 200), (32, 3, 4000), (128, 40, 333)])
+def test_large_scores_in_float16(D, T, S):
+    """Scores of hundreds, one key takes all; equal maps; lam of either sign."""
+    q, k, v, lam, do = da_inputs(gen(23 + D), 2, T, S, 4, 2, D, HF)
+    da_case((q * 16).to(HF), (k * 4).to(HF), v, lam, do, causal=True, scale=0.25)
+    q[:, :, :, 1], k[:, :, :, 1] = q[:, :, :, 0], k[:, :, :, 0]
+    da_case(q, k, v, torch.ones_like(lam), do)
 
 
 # ---------------------------------------------------------------------------------------------- backward
@@ -152,6 +177,39 @@ def test_float16_small_values_keep_the_row_sums():
     ref = da_ref(q, k, v, lam, do, False, 1 / 8, None, None)
     assert float(ref["dq"][0].abs().mean()) > 2.0 ** -12            # far above float16's smallest step
     da_case(q, k, v, lam, do)
+
+
+# ---------------------------------------------------------------------------------------------- lengths and splits
+@pytest.mark.parametrize("dt,D,T", [(BF, 32, 1), (HF, 64, 1), (BF, 128, 1), (HF, 32, 20), (BF, 64, 25)])
+def test_split_keys_with_lengths(dt, D, T):
+    """New tokens over caches of different lengths with several key splits a request (39, 32 and fewer: both forms of their
+    join), splits without a key, sequences without one, and NaN behind the ends."""
+    B, S, H, Hkv = 8, 5000, 4, 2
+    q, k, v, lam, do = da_inputs(gen(300 + D), B, T, S, H, Hkv, D, dt)
+    kv = torch.tensor([0, 1, 31, 33, 5000, 9999, 2600, 128], device="cuda", dtype=torch.int32)
+    for b in range(B):
+        k[b, min(S, int(kv[b])):] = math.nan
+        v[b, min(S, int(kv[b])):] = math.nan
+    out, (dq, dk, dv, _) = da_case(q, k, v, lam, do, causal=T == 1, kv_lens=kv)
+    assert not out[0].any() and not dq[0].any() and not dk[2, 31:].any() and not dv[7, 128:].any()
+
+
+@pytest.mark.parametrize("dt,D,causal,full", [(BF, 64, True, 600), (HF, 32, True, 600), (BF, 128, True, 600), (HF, 64, False, 600),
+                                              (BF, 32, True, 640)])
+def test_split_rows_with_lengths(dt, D, causal, full):
+    """A padded training batch whose rows are split for dK and dV: splits that begin behind a short sequence's end, a sequence
+    of no position, of a few, of fewer positions than keys; NaN behind the ends."""
+    B, H, Hkv = 5, 4, 1
+    T = S = full
+    q, k, v, lam, do = da_inputs(gen(400 + D), B, T, S, H, Hkv, D, dt)
+    lens = torch.tensor([0, full, 5, 333, 40], device="cuda", dtype=torch.int32)
+    ql = torch.tensor([0, full, 5, 333, 7], device="cuda", dtype=torch.int32)
+    for b in range(B):
+        k[b, int(lens[b]):] = math.nan
+        v[b, int(lens[b]):] = math.nan
+        q[b, int(ql[b]):] = math.nan
+    out, (dq, dk, dv, _) = da_case(q, k, v, lam, do, causal=causal, q_lens=ql, kv_lens=lens)
+    assert not out[0].any() and not dk[0].any() and not dv[2, 5:].any() and not dq[4, 7:].any()
 
 
 # ---------------------------------------------------------------------------------------------- Newton-Schulz
