@@ -546,11 +546,12 @@ class FusedAdamW:
 
 
 def muon_keys(arch_order, shapes, kind, n_dense_grad, offsets):
-    """The parameters that Muon takes: the 2-D dense weights that map features to features.  Tables, per-feature embeddings and
-    position biases (rows are looked up, not multiplied), single-output heads and vectors stay with AdamW."""
+    """The parameters that Muon takes: the 2-D dense weights that map features to features.  Tables, per-feature embeddings (num_embed's
+    bias has a row a feature too) and position biases (rows are looked up or added, not multiplied), single-output heads and vectors
+    stay with AdamW."""
     return [k for k in arch_order
             if kind[k] == "dense" and offsets[k] < n_dense_grad and len(shapes[k]) == 2 and min(shapes[k]) >= 2
-            and k not in ("num_embed.weight", "mask_embed.weight") and not k.endswith("pbias.rel.weight")]
+            and k.endswith("weight") and k not in ("num_embed.weight", "mask_embed.weight") and not k.endswith("pbias.rel.weight")]
 
 
 class FusedMuon(FusedAdamW):
