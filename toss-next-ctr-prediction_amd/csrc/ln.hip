@@ -3,7 +3,9 @@
 //   dx = rstd (g - mean_n(g) - xhat mean_n(g xhat)),   dw = sum_m dy xhat,   db = sum_m dy
 // Statistics, sums and partial gradients are fp32 whatever the rows' type; the variance is of the centred values, which
 // stay in registers, so no E[x^2] - mean^2 cancels.  Bound by HBM: the forward pass reads x and writes y, the backward
-// reads x and dy and writes dx; nothing is read twice.
+// reads x and dy and writes dx, each once up to 16384 columns (wider rows are read again for each sum).  The backward also writes
+// and reads 16 N bytes a workgroup of partial weight gradients: nothing beside many rows, but more than the rows themselves
+// where wide rows are few (1024 x 4096 bf16: 67 MB written and read beside 25).
 //
 // TPR threads own a row, thread t its 8-element vectors t, t + TPR, ... (V of them): 16 bytes a lane for the 16-bit
 // types, at whatever alignment the row has (a row of odd width starts at any element).  TPR is the smallest of
@@ -292,9 +294,10 @@ int ln_tpr(int N) {
 int ln_parts(long M, int N) {
   if (N > LN_WIDE) return (int)std::min<long>(std::max<long>(M, 1), 64);
   const int tpr = ln_tpr(N), rpb = std::max(256, tpr) / tpr;
-  // up to eight rows in turn, one launch: 64 x 256 takes 12.1 us a call in a loop and 27.9 alone; a row at a time and a join
-  // 15.4 and 26.1
-  if (tpr <= 64 && M <= 8L * rpb) return 1;
+  // Rows in turn in one block, or a row at a time and a join.  The launch saved is 2.5 us of the host's (a call in a loop 12.7 us
+  // against 15.2 at every size); the kernels alone take, in us, for 4 / 8 / 16 rows in turn (and with a join): 32 columns 6.7 / 9.0 /
+  // 13.7 (6.9), 256: 6.0 / 8.8 / 14.4 (6.2), 512: 5.4 / 8.4 / 14.4 (5.6), 1024: 7.7 / 12.4 / 21.6 (6.6)
+  if (tpr <= 64 && M <= (N <= 512 ? 8L : 4L) * rpb) return 1;
   return (int)std::min<long>(std::max<long>(1, (M + rpb - 1) / rpb), tpr > 256 ? 512 : 1024);
 }
 
