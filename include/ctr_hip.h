@@ -707,9 +707,9 @@ int ctr_diffattn_bwd(const ctr_diffattn_t* p, const void* dout, long g_sb, long 
 
 /* ---- Newton-Schulz orthogonalisation of a list of matrices                                    (newton_schulz.hip)
  * X_0 = G / (||G||_F + eps); `steps` times X <- (a I + b A + c A^2) X, A = X X^T (of the transpose when there are more rows
- * than columns).  src / dst of type 0 fp32, 1 bf16, 2 fp16, row strides in elements; computed to fp32's accuracy.
- * The list is host memory and is read during the call only.  Coefficients under which a singular value could leave
- * [0, 7.5] are refused.                                                                                  */
+ * than columns).  src / dst of type 0 fp32, 1 bf16, 2 fp16, row strides in elements; computed to fp32's accuracy in
+ * the norm whatever the type (an element is held to 2^-22 of itself or 2^-37 of the norm, whichever is more).  The list is host
+ * memory and is read during the call only.  Coefficients under which a singular value could leave [0, 7.5] are refused.  */
 typedef struct {
   const void* src;
   void* dst;

@@ -246,9 +246,10 @@ struct Seq {
 // A pair of waves owns 32 rows, one of them each map: nothing but the value tile's reads is done twice, a wave's
 // accumulators are half as many, and three (D = 64) or two (D = 128) waves share a SIMD, so that one's exponentials run
 // under another's products.  RG pairs a workgroup.  Two 16-bit terms of P make 20 D operations a pair of the 12 D that the
-// definition has; the exponentials and their packing take as long as the products and hide only in part.  Measured: causal
-// 2 x 4096, 16 over 4 heads, D = 64, bf16: 336 us, 0.22 PFLOP/s of the definition's, 0.37 issued; 1531 rows on 5627 keys, 16
-// over 8 heads, D = 128, fp16: 326 us, 0.56 and 0.93 PFLOP/s.  One token on 131072 keys, 8 over 2 heads, D = 128: 42 us, 6.4 TB/s.
+// definition has; the exponentials and their packing hide under the products only in part: of a compute unit's busy cycles the
+// matrix unit works in 59 % and the VALU issues in 68 % at D = 64, 52 and 37 % at D = 128.  Measured: causal 2 x 4096, 16 over 4
+// heads, D = 64, bf16: 330 - 339 us, 0.61 PFLOP/s of the definition's, 1.01 issued; 1531 rows on 5627 keys, 16 over 8 heads,
+// D = 128, fp16: 326 us, 0.56 and 0.94 PFLOP/s.  One token on 131072 keys, 8 over 2 heads, D = 128, bf16: 42 us, 6.4 TB/s.
 // Workgroups: (batch, key head) fastest, so that the eight XCDs, which take workgroups in turn, each keep few heads'
 // keys in their L2; then the splits, then the row tiles, the causally longest first.
 template <typename T, int D, int RG>
@@ -522,7 +523,8 @@ __device__ __forceinline__ void add_cols(uint32_t base, const typename Vec<T>::v
 }
 
 // dQ: a wave owns 32 rows, walks the keys; also the rows' statistics for the dK / dV kernel.  Bound by the products and the
-// exponentials in turn, two waves a SIMD (D <= 64): 256 us at 2 x 4096 causal, 16 over 4 heads, D = 64, bf16.
+// exponentials in turn, two waves a SIMD (D <= 64): 253 - 265 us at 2 x 4096 causal, 16 over 4 heads, D = 64, bf16 (matrix unit
+// 41 %, VALU 59 % of the busy cycles).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 128 ? 1 : 2) void da_bwd_q(const DaArgs a) {
   constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, TILE = Stage<T, D, NW>::TILE;
@@ -682,8 +684,9 @@ __global__ __launch_bounds__(1024) void da_dlam(const DaArgs a) { head_dlam(a, b
 // the same number of matrix instructions each: the first wave forms the maps and dV = (P_1 - lam P_2)^T dO, the second
 // dP, dS and dK_c = dS_c^T Q_c; the probabilities pass from one to the other through LDS in fp32, once a tile.  Each so
 // holds half of the accumulators and three waves (two at D = 128) fit a SIMD: one's exponentials run under the other's products.
-// Bound by the two barriers a tile and the pass through LDS: 490 us at 2 x 4096 causal, 16 over 4 heads, D = 64, bf16, where a
-// wave that did a key's whole work alone took 905 (its accumulators leave one wave a SIMD).
+// Bound by the two barriers a tile and the pass through LDS (matrix unit 28 %, VALU 40 % of the busy cycles): 435 - 480 us at
+// 2 x 4096 causal, 16 over 4 heads, D = 64, bf16, where a wave that did a key's whole work alone took 905 (its accumulators leave
+// one wave a SIMD).
 template <typename T, int D, int NP>
 __global__ __launch_bounds__(128 * NP, D == 128 ? 2 : 3) void da_bwd_kv(const DaArgs a) {
   constexpr int DV = 2 * D, KQ = D / 16, KV = DV / 16, NQ = D / 32, NO = DV / 32, NW = 2 * NP, TILE = Stage<T, D, NW>::TILE;

@@ -2,16 +2,17 @@
 //   X_0 = G / (||G||_F + eps)  (transposed when it has more rows than columns: m <= n below)
 //   A = X X^T,   W = a I + b A + c A^2,   X <- W X        (`steps` times)
 //
-// Arithmetic.  X, A and W are kept as two fp16 planes, hi = fp16(s v) and lo = fp16(s v - hi) with s a power of two that
-// keeps lo out of fp16's subnormals (X: 2^12, A and W: 2^10; the host refuses coefficients under which a singular value
-// of X could pass 8 or one of W 32, the planes' range): 22 mantissa bits and a sign of lo, which is fp32's step to within
-// a factor of two.  A product of two such values is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 with fp32
+// Arithmetic.  X, A and W are kept as two fp16 planes, hi = fp16(s v) and lo = fp16(s v - hi) with s a power of two as large
+// as the planes' range allows (X: 2^12, A and W: 2^10; the host refuses coefficients under which a singular value of X could
+// pass 8 or one of W 32): 22 mantissa bits and a sign of lo, which is fp32's step to within a factor of two, for elements of X
+// from 2^-15 of its norm up, and an absolute 2^-37 of the norm below, where lo is subnormal (elements under 2^-26 so keep fewer
+// bits than a 16-bit input has; in the norm it counts from 65536 x 65536 on).  A product of two such values is hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 with fp32
 // accumulation; the lo lo term is 2^-24 of it.  Three fp16 products cost 3/16 of one fp32 matrix instruction's time, so
 // this is fp32's accuracy at up to five times its rate.  16-bit accuracy would not do: the polynomial multiplies the error
 // of a small singular value by a (3.44) a step, 485 times in five.  Nor would the hi parts do for a bf16 result's last step (2048 x
 // 8192: 1815 us instead of 1942): roundings of matrices with structure do not average out, all ones of 150 x 333 came out 1.2 half
-// steps of bf16 off before their own rounding.  The squares of the norm are summed in fp64, where no
-// fp32 input overflows or vanishes.
+// steps of bf16 off before their own rounding.  The squares of the norm are summed in fp64, where no fp32 input overflows or
+// vanishes.
 #include <algorithm>
 #include <atomic>
 
@@ -498,8 +499,10 @@ __global__ __launch_bounds__(512, 2) void ns_apply(const NsArgs p, int buf, int 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // One workgroup of eight waves holds a matrix: X's planes, and A's (W's after it, in the same place), stay in LDS for all
-// steps, so a list of encoder matrices is one launch.  Bound by the chain of barriers, four a step: 36 us for five steps of
-// twelve matrices of 32 x 32 to 384 x 32, one compute unit each.
+// steps, so a list of encoder matrices is one launch.  Bound by the latency of a chain, not by a rate: of a step's phases (A, A A,
+// W X and the planes' stores) each waits for the last, six barriers a step up to 64 rows and five above, and A A's one tile of
+// 32 rows keeps one wave of the eight busy: 36 us for five steps of twelve matrices of 32 x 32 to 384 x 32, one compute unit each
+// (over 1 us a barrier, so it is not the barriers alone; the phases were not timed apart).
 struct NsSmallArgs {
   float a, b, c, eps;
   int steps;

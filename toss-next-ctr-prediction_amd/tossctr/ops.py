@@ -3,8 +3,9 @@ the Newton-Schulz orthogonalisation of a Muon update (csrc/newton_schulz.hip).
 
 ``layer_norm`` and ``diff_attention`` are differentiable; their ``*_fwd`` / ``*_bwd`` forms are the two passes without
 autograd, for serving, for hand-written training steps and for HIP graphs: a differentiable call under capture is refused, and
-the backward pass of an eager one is not to be captured (torch's engine ties it to the eager call's stream).  All of them run on the current stream of their tensors' device, take
-their workspace from torch's allocator at each call (a captured graph so keeps its own) and never synchronise.
+the backward pass of an eager one is not to be captured (torch's engine ties it to the eager call's stream).  All of them run on
+the current stream of their tensors' device, take their workspace from torch's allocator at each call (a captured graph so keeps
+its own) and never synchronise.
 """
 from __future__ import annotations
 
@@ -218,7 +219,8 @@ def diff_attention_fwd(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_l
     others from a copy.  scale: 1 / sqrt(D) unless given.  q_lens / kv_lens: (B,) int32 device tensors, the valid
     positions and keys of each sequence, held to [0, T] / [0, S]; what stands behind them does not count.  causal: position t
     sees the keys up to t + kv_len - q_len, so one new token (T = 1) sees its whole cache.  Rows that see no key, and
-    positions behind q_lens, are zeros.  ``saved`` is for ``diff_attention_bwd`` (None with ``save=False``)."""
+    positions behind q_lens, are zeros.  A probability is held to two 16-bit terms (2^-16 of itself, float16 2^-22, there at least
+    2^-39 of its row's largest).  ``saved`` is for ``diff_attention_bwd`` (None with ``save=False``)."""
     a, keep = _attn_args("diff_attention", q, k, v, lam, causal, scale, q_lens, kv_lens)
     out = q.new_empty((a.B, a.T, a.H, 2 * a.D))
     saved = None
@@ -237,7 +239,8 @@ def diff_attention_fwd(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_l
 
 
 def diff_attention_bwd(dout, q, k, v, lam, out, saved, causal=False, scale=None, q_lens=None, kv_lens=None):
-    """(dq, dk, dv, dlam) of ``diff_attention_fwd``, given its out and saved and the same other arguments."""
+    """(dq, dk, dv, dlam) of ``diff_attention_fwd``, given its out and saved and the same other arguments.  dS and P_1 - lam P_2 are
+    rounded once to the inputs' type, in float16 held to at least 2^-36 of the row's (dq) or key's (dk, dv) largest."""
     a, keep = _attn_args("diff_attention_bwd", q, k, v, lam, causal, scale, q_lens, kv_lens)
     shape = (a.B, a.T, a.H, 2 * a.D)
     if saved is None:
@@ -289,8 +292,8 @@ def diff_attention(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_lens=
 def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """Orthogonalised matrices: X = G / (||G||_F + eps), then ``steps`` times X <- (a I + b A + c A^2) X with A = X X^T (of
     the transpose when G has more rows than columns).  mats: a matrix, a batch (..., m, n) or a list of matrices of any
-    shapes and one type (float32, bfloat16, float16); the result likewise.  Computed to float32's accuracy whatever the
-    type.  Coefficients under which a singular value could leave [0, 7.5] are refused."""
+    shapes and one type (float32, bfloat16, float16); the result likewise.  Computed to float32's accuracy in the norm
+    whatever the type (an element is held to 2^-22 of itself or 2^-37 of the norm, whichever is more).  Coefficients under which a singular value could leave [0, 7.5] are refused."""
     single = isinstance(mats, torch.Tensor)
     lst = [mats] if single else list(mats)
     if not lst:
