@@ -919,7 +919,7 @@ bool da_wide(long rows) { return rows > 32; }
 // Key splits that give every compute unit two workgroups of four waves, or of two as many as its LDS takes, with at least 128
 // keys each
 int da_splits(const ctr_diffattn_t* p) {
-  const int R = p->T * (p->H / p->Hkv);
+  const long R = (long)p->T * (p->H / p->Hkv);
   const bool wide = da_wide(R);
   const long blocks = (long)cdiv(R, wide ? 64 : 32) * p->B * p->Hkv;
   return (int)std::max<long>(1, std::min<long>((wide || p->D == 128 ? 512 : 1024) / std::max<long>(1, blocks), p->S / 128));
