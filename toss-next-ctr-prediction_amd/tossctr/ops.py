@@ -292,8 +292,9 @@ def diff_attention(q, k, v, lam, causal=False, scale=None, q_lens=None, kv_lens=
 def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """Orthogonalised matrices: X = G / (||G||_F + eps), then ``steps`` times X <- (a I + b A + c A^2) X with A = X X^T (of
     the transpose when G has more rows than columns).  mats: a matrix, a batch (..., m, n) or a list of matrices of any
-    shapes and one type (float32, bfloat16, float16); the result likewise.  Computed to float32's accuracy in the norm
-    whatever the type (an element is held to 2^-22 of itself or 2^-37 of the norm, whichever is more).  Coefficients under which a singular value could leave [0, 7.5] are refused."""
+    shapes (sides up to 65536) and one type (float32, bfloat16, float16); the result likewise.  Computed to float32's accuracy in the norm
+    whatever the type (an element is held to 2^-22 of itself or 2^-37 of the norm, whichever is more).  Coefficients
+    under which a singular value could leave [0, 7.5] are refused."""
     single = isinstance(mats, torch.Tensor)
     lst = [mats] if single else list(mats)
     if not lst:
